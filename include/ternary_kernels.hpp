@@ -176,4 +176,38 @@ inline void copy_to_kv_cache(const half *k, const half *v, half *k_cache, half *
                                      n_kv_heads, head_dim, seq_len, start_pos, max_seq_len, stream));
 }
 
+// The operators around attention that the reference does not have in this form; no counterpart in include/kernels.cuh
+// (its rope_forward, copy_to_kv_cache and attention_forward work on fp16 caches and one start position). The structs are
+// those of tllm_ternary.h and live in host memory.
+inline void rotary_forward(const half *q, const half *k, half *q_out, half *k_out, int64_t q_stride, int64_t k_stride,
+                           int64_t q_out_stride, int64_t k_out_stride, const int *positions, int n_tokens, int n_heads,
+                           int n_kv_heads, int head_dim, const tllm_rotary_config &config, hipStream_t stream = 0) {
+    report("rotary_forward",
+           tllm_rotary_f16(reinterpret_cast<const uint16_t *>(q), reinterpret_cast<const uint16_t *>(k),
+                           reinterpret_cast<uint16_t *>(q_out), reinterpret_cast<uint16_t *>(k_out), q_stride, k_stride,
+                           q_out_stride, k_out_stride, positions, n_tokens, n_heads, n_kv_heads, head_dim, &config, stream));
+}
+
+inline void kv4_append(const half *k, const half *v, int64_t k_stride, int64_t v_stride, const tllm_kv4_cache &cache,
+                       const tllm_kv4_batch &batch, hipStream_t stream = 0) {
+    report("kv4_append", tllm_kv4_append_f16(reinterpret_cast<const uint16_t *>(k), reinterpret_cast<const uint16_t *>(v),
+                                             k_stride, v_stride, &cache, &batch, stream));
+}
+
+inline void kv4_read(half *k, half *v, int64_t k_stride, int64_t v_stride, const tllm_kv4_cache &cache,
+                     const tllm_kv4_batch &batch, hipStream_t stream = 0) {
+    report("kv4_read", tllm_kv4_read_f16(reinterpret_cast<uint16_t *>(k), reinterpret_cast<uint16_t *>(v), k_stride, v_stride,
+                                         &cache, &batch, stream));
+}
+
+inline void attention_kv4_forward(const half *q, half *output, int64_t q_stride, int64_t output_stride,
+                                  const tllm_kv4_cache &cache, const tllm_kv4_batch &batch, int n_heads, int max_query,
+                                  int max_length, float scale, int window, void *workspace, int64_t workspace_bytes,
+                                  hipStream_t stream = 0) {
+    report("attention_kv4_forward",
+           tllm_attention_kv4_f16(reinterpret_cast<const uint16_t *>(q), reinterpret_cast<uint16_t *>(output), q_stride,
+                                  output_stride, &cache, &batch, n_heads, max_query, max_length, scale, window, workspace,
+                                  workspace_bytes, stream));
+}
+
 }  // namespace ternary

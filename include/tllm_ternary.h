@@ -32,11 +32,11 @@ enum {
     TLLM_ERR_BAD_SHAPE = -2,    /* rows/cols/M/N/K/n < 1, or cols % 32 != 0 */
     TLLM_ERR_BAD_GROUP = -3,    /* group_size < 32, group_size % 32 != 0 or cols % group_size != 0 */
     TLLM_ERR_TOO_LARGE = -4,    /* an element count does not fit the index type, or exceeds a stated limit */
-    TLLM_ERR_ALIAS = -5,        /* output overlaps the activation input */
+    TLLM_ERR_ALIAS = -5,        /* an output overlaps an input or another output */
     TLLM_ERR_BAD_PLAN = -6,     /* plan handle is NULL, count < 1, batch out of range, or a pair / prologue rule is broken */
     TLLM_ERR_MISALIGNED = -7,   /* masks/activations not 16-byte aligned, scales/outputs not 2-byte aligned */
     /* -8 and -9 belong to tllm_model_file.h */
-    TLLM_ERR_SCRATCH_TOO_SMALL = -10, /* tllm_ternary_gemm_f16_static: the shape needs more exchange memory than the fixed scratch */
+    TLLM_ERR_SCRATCH_TOO_SMALL = -10, /* tllm_ternary_gemm_f16_static: the shape needs more exchange memory than the fixed scratch; tllm_attention_kv4_f16: workspace too small */
     TLLM_ERR_STAGE_TIMEOUT = -11      /* tllm_linear_plan_status: a launch of a staged plan gave up waiting between two stages */
 };
 
@@ -259,6 +259,130 @@ int tllm_embedding_lookup_f16(const uint16_t *table, const int32_t *indices, uin
 int tllm_copy_to_kv_cache_f16(const uint16_t *k, const uint16_t *v, uint16_t *k_cache,
                               uint16_t *v_cache, int batch, int n_kv_heads, int head_dim,
                               int seq_len, int start_pos, int max_seq_len, tllm_stream_t stream);
+
+/*
+ * Rotary position embedding for rows of any positions, beside tllm_rope_f16 (interleaved pairs, one start position,
+ * whole heads): a position per row, both pair layouts, part of the head, rates scaled for contexts longer than the
+ * trained one, rows with a stride (q and k inside the rows of one q/k/v projection).
+ * q is fp16 [n_tokens, n_heads, head_dim], k [n_tokens, n_kv_heads, head_dim]; *_stride: elements between two rows, heads
+ * lie next to each other. positions: int32 [n_tokens] on the device, any value. n_kv_heads 0: no k (k, k_out may be NULL).
+ * Pair i of a head (i < rotary_dim / 2) is (2i, 2i + 1) in the interleaved layout, (i, i + rotary_dim / 2) in the half
+ * layout:  (x0, x1) -> magnitude * (x0 cos - x1 sin, x0 sin + x1 cos)  of the angle position * w_i; dims from rotary_dim
+ * on are copied. w_i = theta^(-2i / rotary_dim), scaled:
+ *   LINEAR  w_i / factor
+ *   NTK     theta becomes theta * factor^(rotary_dim / (rotary_dim - 2))
+ *   BANDED  b w_i + (1 - b) w_i / factor,  b = (turns_i - low_turns) / (high_turns - low_turns) kept in 0..1, turns_i =
+ *           original_length w_i / (2 pi): fast pairs stay, slow ones are interpolated, between them by their turns
+ *   YARN    b w_i + (1 - b) w_i / factor,  b = 1 - (i - i0) / max(i1 - i0, 0.001) kept in 0..1, i0 = max(0, floor(index(
+ *           high_turns))), i1 = min(rotary_dim - 1, ceil(index(low_turns))), index(t) = the i whose pair makes t turns
+ *           over original_length: between them by their index
+ * Angles are formed in fp64 and reduced to a fraction of a turn there; fp32 arithmetic, one rounding to fp16. q_out / k_out
+ * may be q / k with the same stride (in place); any other overlap of an output with an input or the other output is
+ * TLLM_ERR_ALIAS. config is a HOST pointer. Limits: rotary_dim even, 2..head_dim (from 4 for NTK); head_dim <= 1024, heads <= 1024,
+ * n_tokens < 2^24. No counterpart in the reference beyond kernels/rope.cu:22-104, which tllm_rope_f16 replaces.
+ */
+enum { TLLM_ROTARY_INTERLEAVED = 0, TLLM_ROTARY_HALF = 1 };
+enum { TLLM_ROTARY_NONE = 0, TLLM_ROTARY_LINEAR = 1, TLLM_ROTARY_NTK = 2, TLLM_ROTARY_BANDED = 3, TLLM_ROTARY_YARN = 4 };
+typedef struct tllm_rotary_config {
+    int32_t rotary_dim;
+    int32_t layout;  /* TLLM_ROTARY_INTERLEAVED or TLLM_ROTARY_HALF */
+    int32_t scaling; /* TLLM_ROTARY_NONE .. TLLM_ROTARY_YARN */
+    int32_t original_length; /* BANDED, YARN: trained context, >= 1 */
+    double theta;    /* > 0; > 1 for YARN */
+    double factor;   /* every scaling but NONE: > 0 */
+    double low_turns, high_turns; /* BANDED, YARN: 0 < low_turns < high_turns */
+    double magnitude; /* cosines and sines are multiplied by it (1 unless the scaling asks for more); finite */
+} tllm_rotary_config;
+int tllm_rotary_f16(const uint16_t *q, const uint16_t *k, uint16_t *q_out, uint16_t *k_out, int64_t q_stride,
+                    int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride, const int32_t *positions, int n_tokens,
+                    int n_heads, int n_kv_heads, int head_dim, const tllm_rotary_config *config, tllm_stream_t stream);
+
+/*
+ * A key/value cache held in 4 bits, in pages (5 bits per value with its steps and minima; the fp16 cache of
+ * tllm_copy_to_kv_cache_f16 takes 16). A row (one token, one kv head) is cut into groups of TLLM_KV4_GROUP dims. A group
+ * holds its minimum m and a step s, both fp16, and a code c in 0..15 per value, which stands for m + s * c.
+ *   k_codes  uint32 [n_pages, n_kv_heads, page_size, head_dim / 8]     dim p*64 + r*32 + q*8 + w*4 + b*2 + a (r, w, b, a < 2,
+ *            q < 4) is nibble 4a + 2b + r of word q*(head_dim/32) + 2p + w: a matrix-core operand of 8 dims of one group is
+ *            two words under one mask, and a lane's words lie next to each other
+ *   v_codes  uint32 [n_pages, n_kv_heads, page_size / 4, head_dim / 8, 4]   dim d of slot t is nibble d % 8 of word
+ *            [t / 4][d / 8][t % 4]: four tokens of 8 dims in 16 bytes
+ *   k_scales, v_scales  fp16 [n_pages, n_kv_heads, head_dim / 32, page_size, 2]   (s, m) per group and slot
+ * All four 16-byte aligned. head_dim 64 or 128, page_size a power of two from 16 on, n_pages * n_kv_heads < 2^31, n_kv_heads <= 1024.
+ * The struct lives in HOST memory, its arrays on the device; it is read during the call only.
+ */
+enum { TLLM_KV4_GROUP = 32 };
+typedef struct tllm_kv4_cache {
+    uint32_t *k_codes;
+    uint16_t *k_scales;
+    uint32_t *v_codes;
+    uint16_t *v_scales;
+    int32_t n_pages;
+    int32_t page_size;
+    int32_t n_kv_heads;
+    int32_t head_dim;
+} tllm_kv4_cache;
+/*
+ * The rows of a step: those of sequence b are query_starts[b] .. query_starts[b + 1] - 1 (ascending from 0; a sequence may
+ * have none), and they are its LAST positions: row query_starts[b + 1] - 1 - i is position lengths[b] - 1 - i. lengths
+ * therefore counts the rows of this step too. Position t of sequence b lies in page page_table[b, t / page_size]; an entry
+ * outside 0 .. n_pages - 1 (-1, say) is no page. HOST struct of DEVICE arrays (int32): query_starts [batch + 1], lengths
+ * [batch], page_table [batch, table_width]. n_tokens: rows of the row arrays; rows behind the last sequence are neither
+ * read nor written. The arrays' contents are not seen by the host and cannot be rejected: whatever they hold, the kernels
+ * stay inside the arrays as described. Limits: batch < 2^16, n_tokens < 2^24, table_width * page_size < 2^31.
+ */
+typedef struct tllm_kv4_batch {
+    const int32_t *query_starts;
+    const int32_t *lengths;
+    const int32_t *page_table;
+    int32_t batch;
+    int32_t n_tokens;
+    int32_t table_width;
+} tllm_kv4_batch;
+
+/*
+ * Quantises the rows k, v (fp16 [n_tokens, n_kv_heads, head_dim], *_stride elements between rows) and writes them at their
+ * positions. Per group: m = min, s = fp16((max - m) / 15), c = (x - m) / s rounded to the nearest whole number (of the exact
+ * quotient; ties to even), kept in 0..15, 0 where s is 0. A group with an element that is not finite is stored as s = m =
+ * NaN (what it stands for is NaN). Rows whose position is negative, behind the page table or in no page are dropped, as
+ * tllm_copy_to_kv_cache_f16 drops rows behind the end. A page that is written must belong to one sequence of the batch; what
+ * the pages hold elsewhere stays as it is. Rows 16-byte aligned, strides multiples of 8; k and v may be the same array.
+ */
+int tllm_kv4_append_f16(const uint16_t *k, const uint16_t *v, int64_t k_stride, int64_t v_stride,
+                        const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, tllm_stream_t stream);
+
+/*
+ * The reverse: writes fp16(m + s * c), kept within +-65504, of every row of the batch into k, v (outputs, same layout; k and v
+ * must not overlap).
+ * Rows without a place in the cache become 0. A batch whose rows are all positions reads whole sequences back, e.g. into the
+ * fp16 cache or for another process.
+ */
+int tllm_kv4_read_f16(uint16_t *k, uint16_t *v, int64_t k_stride, int64_t v_stride, const tllm_kv4_cache *cache,
+                      const tllm_kv4_batch *batch, tllm_stream_t stream);
+
+/*
+ * Attention of the rows of a step over the cache: output[r, h] = sum_t p_t v_t, p = softmax over t of scale * q[r, h] . k_t,
+ * with head h reading kv head h / (n_heads / n_kv_heads). A row at position p sees the positions t <= p (its own step's rows
+ * must have been appended) that have a page, with window > 0 only t > p - window. A row that sees nothing becomes 0.
+ * Positions that a row does not see never reach its result, whatever they hold (NaN too). q and output are fp16 [n_tokens,
+ * n_heads, head_dim] with row strides (multiples of 8, 16-byte aligned rows). One token per sequence, some (drafts) and whole
+ * prompts are the same call; sequences of a batch may differ in it.
+ * max_query and max_length are upper bounds the host knows: rows of a sequence from max_query on are left as they were, positions from
+ * max_length on are not seen. They size the launch, so tight ones are faster; for a captured graph take the largest of
+ * its replays. Scores, softmax statistics and sums are fp32, products fp16 x fp16 with exact fp32 accumulation; no atomics:
+ * the same call gives the same bits.
+ * workspace: tllm_attention_kv4_workspace_bytes() bytes of device memory, 16-byte aligned (NULL when that is 0), used during
+ * the call only, contents do not matter; calls that may overlap in time need one each. TLLM_ERR_SCRATCH_TOO_SMALL if less.
+ * Few rows over long contexts are shared out along the positions and joined through it. It depends on the
+ * sizes and on the current device, not on the arrays' contents. Negative: a TLLM_ERR_* code.
+ * Limits: n_heads a multiple of n_kv_heads, <= 4096; 1 <= max_query, max_length; scale finite.
+ * The reference's counterpart for an fp16 cache is kernels/attention.cu:30-333.
+ */
+int64_t tllm_attention_kv4_workspace_bytes(const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, int n_heads, int max_query,
+                                           int max_length);
+int tllm_attention_kv4_f16(const uint16_t *q, uint16_t *output, int64_t q_stride, int64_t output_stride,
+                           const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, int n_heads, int max_query,
+                           int max_length, float scale, int window, void *workspace, int64_t workspace_bytes,
+                           tllm_stream_t stream);
 
 /*
  * Several independent ternary linears in ONE launch (e.g. q/k/v, gate/up, or a whole

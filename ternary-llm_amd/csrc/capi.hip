@@ -1,4 +1,5 @@
 // The C ABI: argument validation and dispatch. No kernel code lives here.
+#include <cmath>
 #include <new>
 #include <vector>
 
@@ -35,6 +36,79 @@ int check_linear(const Problem &p, int group) {
     return TLLM_OK;
 }
 
+// n rows of `bytes` bytes, `stride` bytes apart.
+struct Rows {
+    const void *at;
+    size_t bytes, stride, n;
+    size_t extent() const { return (n - 1) * stride + bytes; }
+};
+
+// Whether two sets of rows share a byte. Rows of one buffer side by side (the q and k parts of a q/k/v projection) have
+// the same stride and interleave without sharing any.
+bool overlaps(const Rows &a, const Rows &b) {
+    if (!overlaps(a.at, a.extent(), b.at, b.extent())) return false;
+    if (a.stride != b.stride || a.stride == 0) return true;
+    const uintptr_t a0 = reinterpret_cast<uintptr_t>(a.at), b0 = reinterpret_cast<uintptr_t>(b.at);
+    const size_t off = b0 >= a0 ? (b0 - a0) % a.stride : (a.stride - (a0 - b0) % a.stride) % a.stride;
+    return off < a.bytes || a.stride - off < b.bytes;
+}
+
+int check_kv4(const tllm_kv4_cache *c, const tllm_kv4_batch *b, Kv4Cache *cache, Kv4Batch *batch, bool sizes_only = false) {
+    if (!c || !b) return TLLM_ERR_NULL_POINTER;
+    if (!sizes_only) {
+        if (!c->k_codes || !c->k_scales || !c->v_codes || !c->v_scales || !b->query_starts || !b->lengths || !b->page_table)
+            return TLLM_ERR_NULL_POINTER;
+        if (misaligned(c->k_codes, 16) || misaligned(c->k_scales, 16) || misaligned(c->v_codes, 16) || misaligned(c->v_scales, 16) ||
+            misaligned(b->query_starts, 4) || misaligned(b->lengths, 4) || misaligned(b->page_table, 4))
+            return TLLM_ERR_MISALIGNED;
+    }
+    if (c->n_pages < 1 || c->n_kv_heads < 1 || (c->head_dim != 64 && c->head_dim != 128) || c->page_size < 16 ||
+        (c->page_size & (c->page_size - 1)) || b->batch < 1 || b->n_tokens < 1 || b->table_width < 1)
+        return TLLM_ERR_BAD_SHAPE;
+    if ((int64_t)c->n_pages * c->n_kv_heads > INT32_MAX || c->n_kv_heads > 1024 || b->batch >= 1 << 16 || b->n_tokens >= 1 << 24 ||
+        (int64_t)b->table_width * c->page_size > INT32_MAX)
+        return TLLM_ERR_TOO_LARGE;
+    *cache = Kv4Cache{c->k_codes, reinterpret_cast<uint32_t *>(c->k_scales), c->v_codes, reinterpret_cast<uint32_t *>(c->v_scales),
+                      c->n_pages, __builtin_ctz((unsigned)c->page_size), c->n_kv_heads, c->head_dim};
+    *batch = Kv4Batch{b->query_starts, b->lengths, b->page_table, b->batch, b->n_tokens, b->table_width};
+    return TLLM_OK;
+}
+
+// The four arrays of a cache, as byte ranges.
+struct CacheRanges {
+    const void *at[4];
+    size_t bytes[4];
+    explicit CacheRanges(const tllm_kv4_cache &c)
+        : at{c.k_codes, c.v_codes, c.k_scales, c.v_scales} {
+        const size_t values = (size_t)c.n_pages * c.n_kv_heads * c.page_size * c.head_dim;
+        bytes[0] = bytes[1] = values / 2;
+        bytes[2] = bytes[3] = values / TLLM_KV4_GROUP * 4;
+    }
+    bool meet(const void *p, size_t n) const {
+        for (int i = 0; i < 4; i++)
+            if (overlaps(at[i], bytes[i], p, n)) return true;
+        return false;
+    }
+    bool meet_each_other() const {
+        for (int i = 0; i < 4; i++)
+            for (int j = 0; j < i; j++)
+                if (overlaps(at[i], bytes[i], at[j], bytes[j])) return true;
+        return false;
+    }
+};
+// The batch's arrays overlap [p, p + n)?
+bool meets(const tllm_kv4_batch &b, const void *p, size_t n) {
+    return overlaps(b.query_starts, ((size_t)b.batch + 1) * 4, p, n) || overlaps(b.lengths, (size_t)b.batch * 4, p, n) ||
+           overlaps(b.page_table, (size_t)b.batch * b.table_width * 4, p, n);
+}
+
+int check_rows(const void *p, int64_t stride, int64_t width) {
+    if (!p) return TLLM_ERR_NULL_POINTER;
+    if (stride < width || stride >= (int64_t)1 << 31) return TLLM_ERR_BAD_SHAPE;
+    if (misaligned(p, 16) || stride % 8) return TLLM_ERR_MISALIGNED;
+    return TLLM_OK;
+}
+
 int run_linear(const Problem &p, int group, hipStream_t s) {
     if (int e = check_linear(p, group)) return e;
     return (int)dispatch_linear(p, group, s);
@@ -58,10 +132,10 @@ const char *tllm_error_string(int code) {
     switch (code) {
         case TLLM_OK: return "ok";
         case TLLM_ERR_NULL_POINTER: return "a required pointer is NULL";
-        case TLLM_ERR_BAD_SHAPE: return "bad shape: sizes must be >= 1 and cols a multiple of 32";
+        case TLLM_ERR_BAD_SHAPE: return "bad shape or parameter: sizes must be >= 1 and cols a multiple of 32";
         case TLLM_ERR_BAD_GROUP: return "bad group_size: must be a multiple of 32 that divides cols";
         case TLLM_ERR_TOO_LARGE: return "size exceeds the supported maximum";
-        case TLLM_ERR_ALIAS: return "output overlaps the activation input";
+        case TLLM_ERR_ALIAS: return "an output overlaps an input or another output";
         case TLLM_ERR_BAD_PLAN: return "invalid plan: handle, problem count, batch, SwiGLU pair or RMSNorm prologue";
         case TLLM_ERR_MISALIGNED: return "pointer alignment: masks/activations need 16 bytes, fp16 arrays 2";
         case -8: return "file cannot be opened, is truncated, or a write failed";   // TLLM_ERR_IO
@@ -70,7 +144,8 @@ const char *tllm_error_string(int code) {
             return "a launch of a staged plan gave up waiting for a stage (its workgroups were not all running at the same time)";
         case TLLM_ERR_SCRATCH_TOO_SMALL:
             return "the split-K exchange of this GEMM shape needs more than the fixed device scratch of "
-                   "tllm_ternary_gemm_f16_static (TLLM_GEMM_STATIC_SCRATCH_BYTES): use tllm_ternary_gemm_f16";
+                   "tllm_ternary_gemm_f16_static (TLLM_GEMM_STATIC_SCRATCH_BYTES): use tllm_ternary_gemm_f16; or the workspace "
+                   "of tllm_attention_kv4_f16 is smaller than tllm_attention_kv4_workspace_bytes";
         default: return code > 0 ? hipGetErrorString((hipError_t)code) : "unknown error code";
     }
 }
@@ -251,6 +326,145 @@ int tllm_copy_to_kv_cache_f16(const uint16_t *k, const uint16_t *v, uint16_t *k_
         return TLLM_ERR_BAD_SHAPE;
     return (int)tllm::launch_copy_to_kv_cache(k, v, k_cache, v_cache, batch, n_kv_heads, head_dim, seq_len, start_pos,
                                               max_seq_len, (hipStream_t)stream);
+}
+
+int tllm_rotary_f16(const uint16_t *q, const uint16_t *k, uint16_t *q_out, uint16_t *k_out, int64_t q_stride,
+                    int64_t k_stride, int64_t q_out_stride, int64_t k_out_stride, const int32_t *positions, int n_tokens,
+                    int n_heads, int n_kv_heads, int head_dim, const tllm_rotary_config *config, tllm_stream_t stream) {
+    if (!q || !q_out || !positions || !config) return TLLM_ERR_NULL_POINTER;
+    const tllm_rotary_config &c = *config;
+    if (n_tokens < 1 || n_heads < 1 || n_kv_heads < 0 || head_dim < 2 || c.rotary_dim < 2 || c.rotary_dim % 2 || c.rotary_dim > head_dim)
+        return TLLM_ERR_BAD_SHAPE;
+    if (n_kv_heads && (!k || !k_out)) return TLLM_ERR_NULL_POINTER;
+    if (n_tokens >= 1 << 24 || n_heads > 1024 || n_kv_heads > 1024 || head_dim > 1024) return TLLM_ERR_TOO_LARGE;
+    if ((c.layout != TLLM_ROTARY_INTERLEAVED && c.layout != TLLM_ROTARY_HALF) || c.scaling < TLLM_ROTARY_NONE || c.scaling > TLLM_ROTARY_YARN)
+        return TLLM_ERR_BAD_SHAPE;
+    const bool banded = c.scaling == TLLM_ROTARY_BANDED || c.scaling == TLLM_ROTARY_YARN;
+    if (!(c.theta > 0.0) || !std::isfinite(c.theta) || !std::isfinite(c.magnitude)) return TLLM_ERR_BAD_SHAPE;
+    if (c.scaling != TLLM_ROTARY_NONE && (!(c.factor > 0.0) || !std::isfinite(c.factor))) return TLLM_ERR_BAD_SHAPE;
+    if (banded && (c.original_length < 1 || !(c.low_turns > 0.0) || !(c.high_turns > c.low_turns) || !std::isfinite(c.high_turns)))
+        return TLLM_ERR_BAD_SHAPE;
+    if ((c.scaling == TLLM_ROTARY_YARN && !(c.theta > 1.0)) || (c.scaling == TLLM_ROTARY_NTK && c.rotary_dim < 4)) return TLLM_ERR_BAD_SHAPE;
+    const int64_t q_width = (int64_t)n_heads * head_dim, k_width = (int64_t)n_kv_heads * head_dim;
+    const int64_t limit = (int64_t)1 << 31;
+    if (q_stride < q_width || q_out_stride < q_width || q_stride >= limit || q_out_stride >= limit) return TLLM_ERR_BAD_SHAPE;
+    if (n_kv_heads && (k_stride < k_width || k_out_stride < k_width || k_stride >= limit || k_out_stride >= limit)) return TLLM_ERR_BAD_SHAPE;
+    if (tllm::misaligned(q, 2) || tllm::misaligned(q_out, 2) || tllm::misaligned(positions, 4) ||
+        (n_kv_heads && (tllm::misaligned(k, 2) || tllm::misaligned(k_out, 2))))
+        return TLLM_ERR_MISALIGNED;
+    const auto rows = [&](const void *p, int64_t width, int64_t stride) { return tllm::Rows{p, (size_t)width * 2, (size_t)stride * 2, (size_t)n_tokens}; };
+    const tllm::Rows qi = rows(q, q_width, q_stride), qo = rows(q_out, q_width, q_out_stride);
+    const tllm::Rows at = {positions, (size_t)n_tokens * 4, (size_t)n_tokens * 4, 1};
+    if ((q_out != q || q_out_stride != q_stride) && tllm::overlaps(qi, qo)) return TLLM_ERR_ALIAS;
+    if (tllm::overlaps(at, qo)) return TLLM_ERR_ALIAS;
+    if (n_kv_heads) {
+        const tllm::Rows ki = rows(k, k_width, k_stride), ko = rows(k_out, k_width, k_out_stride);
+        if ((k_out != k || k_out_stride != k_stride) && tllm::overlaps(ki, ko)) return TLLM_ERR_ALIAS;
+        if (tllm::overlaps(qo, ki) || tllm::overlaps(ko, qi) || tllm::overlaps(qo, ko) || tllm::overlaps(at, ko)) return TLLM_ERR_ALIAS;
+    }
+    tllm::RotaryArgs a{q, k, q_out, k_out, positions, q_stride, k_stride, q_out_stride, k_out_stride, n_tokens, n_heads, n_kv_heads,
+                       head_dim, c.rotary_dim, c.layout == TLLM_ROTARY_HALF, c.scaling, (float)c.magnitude, std::log2(c.theta),
+                       c.scaling == TLLM_ROTARY_NONE ? 1.0 : 1.0 / c.factor, 0.0, 0.0, 0.0};
+    const double dim = c.rotary_dim, turn = 2.0 * 3.14159265358979323846;
+    if (c.scaling == TLLM_ROTARY_NTK) a.log2_theta += std::log2(c.factor) * dim / (dim - 2.0);
+    if (c.scaling == TLLM_ROTARY_BANDED) {
+        a.turns_per_rate = c.original_length / turn;
+        a.low = c.low_turns;
+        a.inv_width = 1.0 / (c.high_turns - c.low_turns);
+    }
+    if (c.scaling == TLLM_ROTARY_YARN) {
+        const auto index = [&](double turns) { return dim * std::log(c.original_length / (turns * turn)) / (2.0 * std::log(c.theta)); };
+        a.low = std::fmax(0.0, std::floor(index(c.high_turns)));
+        const double high = std::fmin(dim - 1.0, std::ceil(index(c.low_turns)));
+        a.inv_width = 1.0 / std::fmax(high - a.low, 0.001);
+    }
+    return (int)tllm::launch_rotary(a, (hipStream_t)stream);
+}
+
+static int kv4_rows(const uint16_t *k, const uint16_t *v, int64_t k_stride, int64_t v_stride, const tllm_kv4_cache *cache,
+                    const tllm_kv4_batch *batch, bool write_rows, tllm::Kv4Cache *c, tllm::Kv4Batch *b) {
+    if (int e = tllm::check_kv4(cache, batch, c, b)) return e;
+    const int64_t width = (int64_t)c->n_kv_heads * c->head_dim;
+    if (int e = tllm::check_rows(k, k_stride, width)) return e;
+    if (int e = tllm::check_rows(v, v_stride, width)) return e;
+    const tllm::Rows kr{k, (size_t)width * 2, (size_t)k_stride * 2, (size_t)b->n_tokens}, vr{v, (size_t)width * 2, (size_t)v_stride * 2, (size_t)b->n_tokens};
+    const tllm::CacheRanges held(*cache);
+    if (held.meet(k, kr.extent()) || held.meet(v, vr.extent())) return TLLM_ERR_ALIAS;
+    if (write_rows) {
+        if (tllm::overlaps(kr, vr) || tllm::meets(*batch, k, kr.extent()) || tllm::meets(*batch, v, vr.extent())) return TLLM_ERR_ALIAS;
+    } else {
+        if (held.meet_each_other()) return TLLM_ERR_ALIAS;
+        for (int i = 0; i < 4; i++)
+            if (tllm::meets(*batch, held.at[i], held.bytes[i])) return TLLM_ERR_ALIAS;
+    }
+    return TLLM_OK;
+}
+
+int tllm_kv4_append_f16(const uint16_t *k, const uint16_t *v, int64_t k_stride, int64_t v_stride, const tllm_kv4_cache *cache,
+                        const tllm_kv4_batch *batch, tllm_stream_t stream) {
+    tllm::Kv4Cache c;
+    tllm::Kv4Batch b;
+    if (int e = kv4_rows(k, v, k_stride, v_stride, cache, batch, false, &c, &b)) return e;
+    return (int)tllm::launch_kv4_append(c, b, k, v, k_stride, v_stride, (hipStream_t)stream);
+}
+
+int tllm_kv4_read_f16(uint16_t *k, uint16_t *v, int64_t k_stride, int64_t v_stride, const tllm_kv4_cache *cache,
+                      const tllm_kv4_batch *batch, tllm_stream_t stream) {
+    tllm::Kv4Cache c;
+    tllm::Kv4Batch b;
+    if (int e = kv4_rows(k, v, k_stride, v_stride, cache, batch, true, &c, &b)) return e;
+    return (int)tllm::launch_kv4_read(c, b, k, v, k_stride, v_stride, (hipStream_t)stream);
+}
+
+static int attention_kv4_args(const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, int n_heads, int max_query, int max_length,
+                              bool sizes_only, tllm::AttentionKv4Args *a) {
+    if (int e = tllm::check_kv4(cache, batch, &a->cache, &a->batch, sizes_only)) return e;
+    if (n_heads < 1 || n_heads % a->cache.n_kv_heads || max_query < 1 || max_length < 1) return TLLM_ERR_BAD_SHAPE;
+    if (n_heads > 4096) return TLLM_ERR_TOO_LARGE;
+    const int capacity = a->batch.width << a->cache.page_shift;
+    a->n_heads = n_heads;
+    a->max_query = max_query < a->batch.n_tokens ? max_query : a->batch.n_tokens;
+    a->max_length = max_length < capacity ? max_length : capacity;
+    return TLLM_OK;
+}
+
+int64_t tllm_attention_kv4_workspace_bytes(const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, int n_heads, int max_query,
+                                           int max_length) {
+    tllm::AttentionKv4Args a{};
+    if (int e = attention_kv4_args(cache, batch, n_heads, max_query, max_length, true, &a)) return e;
+    return (int64_t)tllm::attention_kv4_workspace(a);
+}
+
+int tllm_attention_kv4_f16(const uint16_t *q, uint16_t *output, int64_t q_stride, int64_t output_stride,
+                           const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, int n_heads, int max_query, int max_length,
+                           float scale, int window, void *workspace, int64_t workspace_bytes, tllm_stream_t stream) {
+    tllm::AttentionKv4Args a{};
+    if (int e = attention_kv4_args(cache, batch, n_heads, max_query, max_length, false, &a)) return e;
+    if (window < 0 || !std::isfinite(scale)) return TLLM_ERR_BAD_SHAPE;
+    const int64_t width = (int64_t)n_heads * a.cache.head_dim;
+    if (int e = tllm::check_rows(q, q_stride, width)) return e;
+    if (int e = tllm::check_rows(output, output_stride, width)) return e;
+    const size_t need = tllm::attention_kv4_workspace(a);
+    if (need) {
+        if (!workspace) return TLLM_ERR_NULL_POINTER;
+        if (workspace_bytes < 0 || (size_t)workspace_bytes < need) return TLLM_ERR_SCRATCH_TOO_SMALL;
+        if (tllm::misaligned(workspace, 16)) return TLLM_ERR_MISALIGNED;
+    }
+    const tllm::Rows qr{q, (size_t)width * 2, (size_t)q_stride * 2, (size_t)a.batch.n_tokens};
+    const tllm::Rows out{output, (size_t)width * 2, (size_t)output_stride * 2, (size_t)a.batch.n_tokens};
+    const tllm::CacheRanges held(*cache);
+    if (tllm::overlaps(qr, out) || held.meet(output, out.extent()) || tllm::meets(*batch, output, out.extent())) return TLLM_ERR_ALIAS;
+    if (need && (held.meet(workspace, need) || tllm::meets(*batch, workspace, need) || tllm::overlaps(workspace, need, q, qr.extent()) ||
+                 tllm::overlaps(workspace, need, output, out.extent())))
+        return TLLM_ERR_ALIAS;
+    a.q = q;
+    a.output = output;
+    a.q_stride = q_stride;
+    a.output_stride = output_stride;
+    a.window = window;
+    a.scale = scale;
+    a.workspace = workspace;
+    return (int)tllm::launch_attention_kv4(a, (hipStream_t)stream);
 }
 
 int tllm_debug_set_tuning(const char *name, int value) {

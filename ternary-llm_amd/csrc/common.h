@@ -147,6 +147,46 @@ hipError_t launch_copy_to_kv_cache(const uint16_t *k, const uint16_t *v, uint16_
                                    int n_kv_heads, int head_dim, int seq_len, int start_pos, int max_seq_len,
                                    hipStream_t s);
 
+// Rotary positions (rotary.hip). Strides in elements between tokens; n_kv_heads 0: no k.
+struct RotaryArgs {
+    const uint16_t *q, *k;
+    uint16_t *q_out, *k_out;
+    const int32_t *positions;
+    int64_t q_stride, k_stride, q_out_stride, k_out_stride;
+    int32_t n_tokens, n_heads, n_kv_heads, head_dim, rotary_dim, half_layout, scaling;
+    float magnitude;
+    // w_i = 2^(-log2_theta 2i / rotary_dim); the scalings blend it with w_i * inv_factor: banded by
+    // (turns_per_rate * w_i - low) * inv_width, YaRN by 1 - (i - low) * inv_width, both kept in 0..1
+    double log2_theta, inv_factor, turns_per_rate, low, inv_width;
+};
+hipError_t launch_rotary(const RotaryArgs &a, hipStream_t s);
+
+// The 4-bit paged key/value cache (kv4.hip) and attention over it (attention_kv4.hip).
+struct Kv4Cache {
+    uint32_t *k_codes, *k_scales, *v_codes, *v_scales;  // scales: one word per group and token, step | minimum << 16
+    int32_t n_pages, page_shift, n_kv_heads, head_dim;
+};
+struct Kv4Batch {
+    const int32_t *starts, *lengths, *table;
+    int32_t batch, n_tokens, width;
+};
+hipError_t launch_kv4_append(const Kv4Cache &c, const Kv4Batch &b, const uint16_t *k, const uint16_t *v, int64_t k_stride,
+                             int64_t v_stride, hipStream_t s);
+hipError_t launch_kv4_read(const Kv4Cache &c, const Kv4Batch &b, uint16_t *k, uint16_t *v, int64_t k_stride, int64_t v_stride,
+                           hipStream_t s);
+struct AttentionKv4Args {
+    Kv4Cache cache;
+    Kv4Batch batch;
+    const uint16_t *q;
+    uint16_t *output;
+    int64_t q_stride, output_stride;
+    int32_t n_heads, max_query, max_length, window;  // window 0: none
+    float scale;
+    void *workspace;
+};
+size_t attention_kv4_workspace(const AttentionKv4Args &a);  // pointers are not looked at
+hipError_t launch_attention_kv4(const AttentionKv4Args &a, hipStream_t s);
+
 // Measurement aid (elementwise.hip): reads `bytes` of device memory once.
 hipError_t launch_read_stream(const void *src, size_t bytes, uint32_t *sink, hipStream_t s);
 

@@ -21,7 +21,8 @@ ABI_SYMBOLS = (
     "tllm_linear_plan_kernel", "tllm_gemm_workspace_reserve", "tllm_gemm_workspace_release",
     "tllm_ternary_gemm_f16_static", "tllm_ternary_gemm_swiglu_f16", "tllm_ternary_gemm_group_f16", "tllm_read_stream", "tllm_ternary_gemm_kernel",
     "tllm_debug_set_tuning", "tllm_debug_get_tuning", "tllm_ternary_linear_int8_f16",
-    "tllm_linear_plan_create_staged", "tllm_linear_plan_status",
+    "tllm_linear_plan_create_staged", "tllm_linear_plan_status", "tllm_rotary_f16", "tllm_kv4_append_f16",
+    "tllm_kv4_read_f16", "tllm_attention_kv4_workspace_bytes", "tllm_attention_kv4_f16",
 )
 # include/tllm_model_file.h
 FILE_ABI_SYMBOLS = (
@@ -41,6 +42,22 @@ class _Problem(C.Structure):
     _fields_ = [("nonzero_masks", C.c_void_p), ("sign_masks", C.c_void_p), ("scales", C.c_void_p),
                 ("input", C.c_void_p), ("output", C.c_void_p), ("rows", C.c_int32),
                 ("cols", C.c_int32), ("batch", C.c_int32), ("flags", C.c_int32)]
+
+
+class _RotaryConfig(C.Structure):
+    _fields_ = [("rotary_dim", C.c_int32), ("layout", C.c_int32), ("scaling", C.c_int32), ("original_length", C.c_int32),
+                ("theta", C.c_double), ("factor", C.c_double), ("low_turns", C.c_double), ("high_turns", C.c_double),
+                ("magnitude", C.c_double)]
+
+
+class _Kv4Cache(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+                ("n_pages", C.c_int32), ("page_size", C.c_int32), ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
+class _Kv4Batch(C.Structure):
+    _fields_ = [("query_starts", C.c_void_p), ("lengths", C.c_void_p), ("page_table", C.c_void_p), ("batch", C.c_int32),
+                ("n_tokens", C.c_int32), ("table_width", C.c_int32)]
 
 
 class FileHeader(C.Structure):
@@ -110,6 +127,14 @@ def lib():
     L.tllm_rope_f16.argtypes = [vp, vp, i, i, i, i, i, i, f, vp]
     L.tllm_embedding_lookup_f16.argtypes = [vp, vp, vp, i, i, vp]
     L.tllm_copy_to_kv_cache_f16.argtypes = [vp, vp, vp, vp, i, i, i, i, i, i, vp]
+    i64 = C.c_int64
+    L.tllm_rotary_f16.argtypes = [vp, vp, vp, vp, i64, i64, i64, i64, vp, i, i, i, i, C.POINTER(_RotaryConfig), vp]
+    cache, batch = C.POINTER(_Kv4Cache), C.POINTER(_Kv4Batch)
+    L.tllm_kv4_append_f16.argtypes = [vp, vp, i64, i64, cache, batch, vp]
+    L.tllm_kv4_read_f16.argtypes = [vp, vp, i64, i64, cache, batch, vp]
+    L.tllm_attention_kv4_workspace_bytes.argtypes = [cache, batch, i, i, i]
+    L.tllm_attention_kv4_workspace_bytes.restype = i64
+    L.tllm_attention_kv4_f16.argtypes = [vp, vp, i64, i64, cache, batch, i, i, i, f, i, vp, i64, vp]
     L.tllm_ternarize_pack_f32.argtypes = [vp, i, i, i, f, vp, vp, vp]
     L.tllm_model_file_open.argtypes = [C.c_char_p, C.POINTER(vp)]
     L.tllm_model_file_close.argtypes = [vp]
@@ -289,6 +314,172 @@ def copy_to_kv_cache(k, v, k_cache, v_cache, batch, n_kv_heads, head_dim, seq_le
     """New k/v rows into the caches at start_pos (reference include/kernels.cuh:72-76)."""
     check(lib().tllm_copy_to_kv_cache_f16(_ptr(k), _ptr(v), _ptr(k_cache), _ptr(v_cache), batch, n_kv_heads, head_dim,
                                           seq_len, start_pos, max_seq_len, _stream(stream)))
+
+
+ROTARY_LAYOUTS = {"interleaved": 0, "half": 1}
+ROTARY_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "banded": 3, "yarn": 4}
+
+
+def _want(cond, text):
+    if not cond:
+        raise ValueError(text)
+
+
+def _rows(t, name, heads=None):
+    """A tensor of rows [n, heads, dim]: fp16, heads next to each other; returns its row stride in elements."""
+    _want(t.dim() == 3 and t.dtype == _float16(), f"{name} must be fp16 [rows, heads, dim]")
+    n, h, d = t.shape
+    stride = t.stride()
+    _want((stride[2] == 1 or d == 1) and (stride[1] == d or h == 1), f"the heads of a row of {name} must lie next to each other")
+    _want(heads is None or h == heads, f"{name} has {h} heads, {heads} are expected")
+    return stride[0] if n > 1 else h * d
+
+
+def _float16():
+    import torch
+    return torch.float16
+
+
+class _on:
+    """Launches go to the device of the tensors: makes it the current one if it is not (the library launches on the
+    current device) and gives the stream to use. A stream that is given must belong to that device."""
+
+    def __init__(self, stream, first, *others):
+        import torch
+        device = first.device
+        _want(first.is_cuda and all(t.device == device for t in others), "the tensors must lie on one GPU")
+        _want(stream is None or stream.device == device, "the stream belongs to another device than the tensors")
+        self.stream = torch.cuda.current_stream(device) if stream is None else stream
+        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return C.c_void_p(self.stream.cuda_stream)
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def rotary(q, k, q_out, k_out, positions, rotary_dim, theta, layout="interleaved", scaling="none", factor=1.0, original_length=8192,
+           low_turns=1.0, high_turns=None, magnitude=1.0, stream=None):
+    """Rotary position embedding beside `rope` (include/tllm_ternary.h, tllm_rotary_f16): a position per row (int32 on the
+    device), layout "interleaved" or "half", the first rotary_dim dims of each head, scaling "none", "linear", "ntk",
+    "banded" or "yarn" (high_turns: 4 for "banded", 32 for "yarn" unless given). q, q_out: fp16 [rows, heads, dim], k, k_out
+    [rows, kv_heads, dim] (or None), rows of any stride; the outputs may be the inputs."""
+    _want(layout in ROTARY_LAYOUTS, f"layout must be one of {sorted(ROTARY_LAYOUTS)}")
+    _want(scaling in ROTARY_SCALINGS, f"scaling must be one of {sorted(ROTARY_SCALINGS)}")
+    _want((k is None) == (k_out is None), "k and k_out come together")
+    n, heads, dim = q.shape
+    strides = [_rows(q, "q"), 0, _rows(q_out, "q_out"), 0]
+    _want(q_out.shape == q.shape, "q_out must have q's shape")
+    kv_heads = 0
+    if k is not None:
+        strides[1], strides[3] = _rows(k, "k"), _rows(k_out, "k_out")
+        kv_heads = k.shape[1]
+        _want(k.shape == k_out.shape and k.shape[0] == n and k.shape[2] == dim, "k and k_out must have q's rows and dim")
+    _want(_is_int32(positions) and positions.shape == (n,), "positions must be a contiguous int32 [rows]")
+    if high_turns is None:
+        high_turns = 32.0 if scaling == "yarn" else 4.0
+    config = _RotaryConfig(rotary_dim, ROTARY_LAYOUTS[layout], ROTARY_SCALINGS[scaling], original_length, theta, factor, low_turns,
+                           high_turns, magnitude)
+    others = (q_out, positions) if k is None else (q_out, positions, k, k_out)
+    with _on(stream, q, *others) as s:
+        check(lib().tllm_rotary_f16(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), *strides, _ptr(positions), n, heads, kv_heads, dim,
+                                    config, s))
+
+
+def _is_int32(t):
+    import torch
+    return t.dtype == torch.int32 and t.is_contiguous()
+
+
+def _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n_tokens):
+    """The two structs of a call from its tensors."""
+    pages, heads, page, words = k_codes.shape
+    dim = words * 8
+    _want(_is_int32(k_codes) and _is_int32(v_codes) and v_codes.shape == (pages, heads, page // 4, words, 4),
+          "codes must be contiguous int32: k [pages, heads, page, dim / 8], v [pages, heads, page / 4, dim / 8, 4]")
+    shape = (pages, heads, dim // 32, page, 2)
+    half = _float16()
+    _want(k_scales.shape == shape and v_scales.shape == shape and k_scales.dtype == half and v_scales.dtype == half
+          and k_scales.is_contiguous() and v_scales.is_contiguous(), "scales must be contiguous fp16 [pages, heads, dim / 32, page, 2]")
+    batch, = lengths.shape
+    _want(_is_int32(query_starts) and _is_int32(lengths) and _is_int32(page_table) and query_starts.shape == (batch + 1,)
+          and page_table.dim() == 2 and page_table.shape[0] == batch,
+          "query_starts [batch + 1], lengths [batch] and page_table [batch, width] must be contiguous int32")
+    return (_Kv4Cache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), pages, page, heads, dim),
+            _Kv4Batch(query_starts.data_ptr(), lengths.data_ptr(), page_table.data_ptr(), batch, n_tokens, page_table.shape[1]))
+
+
+def kv4_cache(n_pages, page_size, n_kv_heads, head_dim, device="cuda"):
+    """(k_codes, k_scales, v_codes, v_scales) of an empty 4-bit paged cache (include/tllm_ternary.h, tllm_kv4_cache)."""
+    import torch
+    _want(n_pages >= 1 and n_kv_heads >= 1 and head_dim in (64, 128) and page_size >= 16 and page_size & (page_size - 1) == 0,
+          "head_dim 64 or 128, page_size a power of two from 16 on")
+    codes = lambda *shape: torch.zeros(n_pages, n_kv_heads, *shape, dtype=torch.int32, device=device)  # noqa: E731
+    scales = lambda: torch.zeros(n_pages, n_kv_heads, head_dim // 32, page_size, 2, dtype=torch.float16, device=device)  # noqa: E731
+    return codes(page_size, head_dim // 8), scales(), codes(page_size // 4, head_dim // 8, 4), scales()
+
+
+def kv4_append(k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, stream=None):
+    """Quantises the rows k, v [rows, kv_heads, dim] to 4 bits and writes them at the last positions of their sequences
+    (include/tllm_ternary.h, tllm_kv4_append_f16; the fp16 counterpart is copy_to_kv_cache)."""
+    cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, k.shape[0])
+    ks, vs = _rows(k, "k", cache.n_kv_heads), _rows(v, "v", cache.n_kv_heads)
+    _want(k.shape == v.shape and k.shape[2] == cache.head_dim, "k and v must be [rows, kv_heads, dim] of the cache")
+    with _on(stream, k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table) as s:
+        check(lib().tllm_kv4_append_f16(_ptr(k), _ptr(v), ks, vs, cache, batch, s))
+
+
+def kv4_read(k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, stream=None):
+    """Writes what the cache holds for the rows of a batch into k, v (fp16 [rows, kv_heads, dim]; tllm_kv4_read_f16)."""
+    cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, k.shape[0])
+    ks, vs = _rows(k, "k", cache.n_kv_heads), _rows(v, "v", cache.n_kv_heads)
+    _want(k.shape == v.shape and k.shape[2] == cache.head_dim, "k and v must be [rows, kv_heads, dim] of the cache")
+    with _on(stream, k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table) as s:
+        check(lib().tllm_kv4_read_f16(_ptr(k), _ptr(v), ks, vs, cache, batch, s))
+
+
+def attention_kv4(q, output, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, max_query, max_length, scale=None,
+                  window=0, workspace=None, stream=None):
+    """Causal attention of the rows q [rows, heads, dim] over the 4-bit cache (include/tllm_ternary.h,
+    tllm_attention_kv4_f16): the rows are the last positions of their sequences and must have been appended. max_query,
+    max_length: upper bounds of the rows and of the cached positions of a sequence. scale: 1 / sqrt(dim) unless given.
+    workspace: a contiguous tensor of attention_kv4_workspace_bytes(...) bytes; without one it is taken from torch's
+    allocator for the time of the call, on the call's stream."""
+    n, heads, dim = q.shape
+    cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n)
+    qs, os_ = _rows(q, "q"), _rows(output, "output")
+    _want(output.shape == q.shape and dim == cache.head_dim, "q and output must be [rows, heads, dim] with the cache's dim")
+    with _on(stream, q, output, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table) as s:
+        L = lib()
+        need = L.tllm_attention_kv4_workspace_bytes(cache, batch, heads, max_query, max_length)
+        if need < 0:
+            check(int(need))
+        if workspace is not None:
+            _want(workspace.device == q.device and workspace.is_contiguous(), "the workspace must be contiguous, on the tensors' GPU")
+            have = workspace.numel() * workspace.element_size()
+        else:
+            have = need
+            if need:
+                import torch
+                with torch.cuda.stream(stream):  # (a stream of its own: the allocator hands the memory out in its order)
+                    workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        check(L.tllm_attention_kv4_f16(_ptr(q), _ptr(output), qs, os_, cache, batch, heads, max_query, max_length,
+                                       dim ** -0.5 if scale is None else scale, window, _ptr(workspace), have, s))
+
+
+def attention_kv4_workspace_bytes(n_heads, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n_rows, max_query,
+                                  max_length):
+    """Bytes of workspace that attention_kv4 uses for these sizes on the current device."""
+    cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n_rows)
+    need = int(lib().tllm_attention_kv4_workspace_bytes(cache, batch, n_heads, max_query, max_length))
+    if need < 0:
+        check(need)
+    return need
 
 
 SWIGLU_GATE = 1  # TLLM_PROBLEM_SWIGLU_GATE
