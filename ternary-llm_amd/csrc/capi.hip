@@ -1,4 +1,5 @@
 // The C ABI: argument validation and dispatch. No kernel code lives here.
+#include <algorithm>
 #include <cmath>
 #include <new>
 #include <vector>
@@ -420,7 +421,7 @@ static int attention_kv4_args(const tllm_kv4_cache *cache, const tllm_kv4_batch 
                               bool sizes_only, tllm::AttentionKv4Args *a) {
     if (int e = tllm::check_kv4(cache, batch, &a->cache, &a->batch, sizes_only)) return e;
     if (n_heads < 1 || n_heads % a->cache.n_kv_heads || max_query < 1 || max_length < 1) return TLLM_ERR_BAD_SHAPE;
-    if (n_heads > 4096) return TLLM_ERR_TOO_LARGE;
+    if (n_heads > 4096 || (int64_t)n_heads * std::min(max_query, a->batch.n_tokens) > 1 << 27) return TLLM_ERR_TOO_LARGE;
     const int capacity = a->batch.width << a->cache.page_shift;
     a->n_heads = n_heads;
     a->max_query = max_query < a->batch.n_tokens ? max_query : a->batch.n_tokens;
@@ -440,7 +441,7 @@ int tllm_attention_kv4_f16(const uint16_t *q, uint16_t *output, int64_t q_stride
                            float scale, int window, void *workspace, int64_t workspace_bytes, tllm_stream_t stream) {
     tllm::AttentionKv4Args a{};
     if (int e = attention_kv4_args(cache, batch, n_heads, max_query, max_length, false, &a)) return e;
-    if (window < 0 || !std::isfinite(scale)) return TLLM_ERR_BAD_SHAPE;
+    if (window < 0 || !(std::fabs(scale) <= 1099511627776.0f)) return TLLM_ERR_BAD_SHAPE;
     const int64_t width = (int64_t)n_heads * a.cache.head_dim;
     if (int e = tllm::check_rows(q, q_stride, width)) return e;
     if (int e = tllm::check_rows(output, output_stride, width)) return e;

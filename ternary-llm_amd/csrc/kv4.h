@@ -1,5 +1,7 @@
 // The 4-bit paged key/value cache as the kernels see it (layout: include/tllm_ternary.h, tllm_kv4_cache).
 #pragma once
+#include <type_traits>
+
 #include "common.h"
 
 namespace tllm {

@@ -87,12 +87,23 @@ def test_attention_refusals():
     assert _attend_call(q=None) == -1 and _attend_call(out=None) == -1 and _attend_call(table=None) == -1
     assert _attend_call(heads=3) == -2 and _attend_call(heads=0) == -2 and _attend_call(mq=0) == -2 and _attend_call(ml=0) == -2
     assert _attend_call(window=-1) == -2 and _attend_call(scale=float("inf")) == -2 and _attend_call(scale=float("nan")) == -2
-    assert _attend_call(heads=4098, qs=1 << 20, os_=1 << 20) == -4
+    assert _attend_call(heads=4098, qs=1 << 20, os_=1 << 20) == -4 and _attend_call(scale=2e12) == -2
+    assert _attend_call(heads=4096, qs=1 << 20, os_=1 << 20, n=1 << 20, mq=1 << 16) == -4
     assert _attend_call(qs=248) == -2 and _attend_call(qs=260) == -7 and _attend_call(out=0x600008) == -7 and _attend_call(dim=32) == -2
     assert _attend_call(out=0x500100) == -5 and _attend_call(out=0x100000) == -5 and _attend_call(lengths=0x600040) == -5
     c, b = _kv4()
     size = tl.lib().tllm_attention_kv4_workspace_bytes
     assert size(c, b, 4, 3, 32) >= 0 and size(c, b, 3, 3, 32) == -2 and size(None, b, 4, 3, 32) == -1
+
+    # one row over a long context is shared out: a workspace is asked for and checked
+    long = dict(pages=2048, page=64, batch=1, n=1, width=2048, kc=0x10000000, ks=0x20000000, vc=0x30000000, vs=0x40000000)
+    need = size(*_kv4(**long), 4, 1, 131072)
+    assert need > 0
+    assert _attend_call(mq=1, ml=131072, ws=None, **long) == -1
+    assert _attend_call(mq=1, ml=131072, wsb=need - 1, **long) == -10 and _attend_call(mq=1, ml=131072, wsb=-1, **long) == -10
+    assert _attend_call(mq=1, ml=131072, ws=0x800004, **long) == -7
+    assert _attend_call(mq=1, ml=131072, ws=0x10000010, **long) == -5 and _attend_call(mq=1, ml=131072, ws=0x500010, **long) == -5
+    assert _attend_call(mq=1, ml=131072, ws=0x600000 - 16, **long) == -5
 
 
 def test_python_refusals():
