@@ -24,35 +24,34 @@ constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr float kEmpty = -1e30f;  // below every score (|q.k| < 2^40, |scale| <= 2^40): no position yet
 constexpr int kHeadroom = 6;      // powers of two that a weight may outgrow its base by before everything is rescaled
 constexpr int kTopPower = 8;      // a base puts the largest weight seen (times its step) at 2^kTopPower
-constexpr int kMostSplits = 128;
 constexpr uint32_t kEvenCodes = 0x000F000Fu, kOddCodes = 0x00F000F0u;
-// The values' codes are brought to c - 8 in ordinary fp16 first: 1024 + c (or 64 + c, from bits 4-7) with one ternary
-// instruction, minus the rest with a packed one. Bare codes would be cheaper by that one, but the matrix unit lines products
-// up by their operands' exponents, of which a subnormal has the smallest however few bits it fills, and cuts what falls off:
-// sums of up to 2^-22 too low, which positive codes add up to 2 sqrt(positions) times what is left of the values in the end
-// (4e-4 of the result at 131072 positions). Scores, sums of 128 products with their signs, do not feel it.
-constexpr uint32_t kEvenBits = 0x64006400u, kOddBits = 0x54005400u;
+// The values' codes are all brought to bits 4-7, and every second position's enter as 15 - c with a negative weight (15 p s
+// goes to the minima's sum). The matrix unit lines products up by their operands' exponents, of which a subnormal has the
+// smallest however few bits it fills, and cuts what falls off: with codes in bits 0-3 sums come out 2^-22 too low, which
+// positive codes add up to 2 sqrt(positions) times what is left of the values in the end (4e-4 of the result at 131072
+// positions). Scores, sums of 128 products with their signs, do not feel it.
+constexpr uint32_t kSecondFlipped = 0xFFFF0000u;
 
 __device__ __forceinline__ float low_half(uint32_t w) { return h2f((uint16_t)w); }
 __device__ __forceinline__ float high_half(uint32_t w) { return h2f((uint16_t)(w >> 16)); }
 
-// What the host and both kernels have to agree on.
-struct SplitPlan {
-    int splits;      // most parts that a row tile's positions are shared out to
-    int row_tiles;   // of max_query rows
-};
-
-// The positions [lo, hi) that some row of a tile sees, and its parts in steps of `step` positions.
-struct Span {
-    int first, steps, per, used;  // first step, steps, steps per part, parts that have any
-    __device__ Span(int lo, int hi, int step, int splits) {
-        first = lo / step;
-        steps = hi > lo ? (hi + step - 1) / step - first : 0;
-        per = (steps + splits - 1) / splits;
-        per = per < kWaves ? kWaves : (per + kWaves - 1) & ~(kWaves - 1);
-        used = (steps + per - 1) / per;
-    }
-};
+// Sums and maxima over the 16 lanes of a quad, in every lane (rotations inside the quad), and over all lanes.
+template <int kBy>
+__device__ __forceinline__ float rotated(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x120 + kBy, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += rotated<8>(v);
+    v += rotated<4>(v);
+    v += rotated<2>(v);
+    return v + rotated<1>(v);
+}
+__device__ __forceinline__ float quad_max(float v) {
+    v = fmaxf(v, rotated<8>(v));
+    v = fmaxf(v, rotated<4>(v));
+    v = fmaxf(v, rotated<2>(v));
+    return fmaxf(v, rotated<1>(v));
+}
 
 // Rows of a sequence, in range whatever the arrays hold.
 struct Sequence {
@@ -71,20 +70,31 @@ __device__ __forceinline__ int window_begin(const AttentionKv4Args &a, int pos) 
 
 // ------------------------------------------------------------------------------------------------- few rows: decode
 //
-// A workgroup takes up to kRows rows (query rows times the heads that share a kv head; kRows 4, 8 or 16) and a part of the
-// positions; its four waves take steps of kStep positions in turn and are joined through LDS at the end, parts through the
-// workspace. Bound: HBM, the cache's 5 bits per value; the work per position has to stay small beside it, above all the
-// work on scores, of which 16 x 16 come out of every matrix instruction however few rows there are. So the row operand
-// repeats its kRows rows, and of kPack = 16 / kRows tiles of 16 positions each quad of lanes keeps the results of its own
-// tile: each of the 64 lanes then has ONE position and four rows of its own (lane = (position t, quad)), steps and minima
-// are one coalesced word per lane and group, and softmax runs on four registers. For the values, weights p s go through LDS ([position][group][row], fp16) and come
-// back transposed (ds_read_b64_tr_b16) with (group, row) pairs as the 16 columns of the operand: one instruction multiplies
-// a row tile's weights of all groups in the set, of which each dim uses its own group's.
+// Bound: HBM, the cache's 5 bits per value; the work per position has to stay small beside it, above all the work on scores,
+// of which 16 x 16 come out of every matrix instruction however few rows there are. So the row operand repeats its kRows
+// rows (query rows times the heads that share a kv head: 4, 8 or 16), and of kPack = 16 / kRows tiles of 16 positions each
+// quad of lanes keeps the results of its own tile: each of the 64 lanes then has ONE position and four rows of its own (lane
+// = (position t, quad)), steps and minima are one coalesced word per lane and group, and softmax runs on four registers. For
+// the values, weights p s go through LDS ([position][group][row], fp16) and come back transposed (ds_read_b64_tr_b16) with
+// (group, row) pairs as the 16 columns of the operand: one instruction multiplies a row tile's weights of all groups in the
+// set, of which each dim uses its own group's.
+//
+// The positions of all sequences are one line of steps, cut into equal pieces, one per workgroup (each kv head its own
+// line): however ragged the batch, all workgroups end together. A piece may end inside a sequence and begin inside another;
+// its stretch of a sequence is a segment. A sequence that lies in one piece is stored at once, the segments of others are
+// joined by a second launch. The four waves of a workgroup take the steps of a segment in turn and meet in LDS.
+struct DecodePlan {
+    int workers;  // workgroups per kv head
+    int tiles;    // row tiles per sequence; row tile t of sequence b is number b * tiles + t of the line
+    int least;    // steps that a piece has at least
+    int alone;    // every workgroup has a whole row tile (no second launch)
+};
+
 template <int kDim, int kRows>
 struct Decode {
     static constexpr int kGroups = kDim / kKvGroup, kWords = kDim / 8;
     static constexpr int kPack = 16 / kRows;
-    static constexpr int kTiles = kRows == 16 ? 2 : 4, kStep = 16 * kTiles, kPasses = kTiles / kPack;
+    static constexpr int kTiles = kRows == 4 ? 4 : 2, kStep = 16 * kTiles, kPasses = kTiles / kPack;
     static constexpr int kColumns = kGroups * kRows < 16 ? 16 : kGroups * kRows;  // of the weights: (group, row)
     static constexpr int kSets = kColumns / 16, kSetGroups = kGroups / kSets;
     static constexpr int kSetWords = 4 * kSetGroups, kLanesPerWord = 16 / kSetWords, kNibbles = 8 / kLanesPerWord;
@@ -92,10 +102,9 @@ struct Decode {
     static constexpr int kWaveBytes = kStep * kRowBytes;
     static constexpr int kJoinBytes = kWaves * kRows * kDim * 4;
     static constexpr int kLds = kWaves * kWaveBytes > kJoinBytes ? kWaves * kWaveBytes : kJoinBytes;
-    static_assert(kWaveBytes >= 64 * (kGroups * 4 + 4) * 4 / 4, "the sums of the minima");
     using KeyWords = typename std::conditional<kGroups == 4, uint4_t, uint2_t>::type;
     struct Places {
-        int block[kTiles], slot[kTiles];  // of each tile of 16 positions: page * n_kv_heads + head, first slot
+        uint32_t block[kTiles], slot[kTiles];  // of each tile of 16 positions: page * n_kv_heads + head, first slot
         uint32_t there;                   // bit i: tile i has a page
     };
     struct Keys {
@@ -107,8 +116,53 @@ struct Decode {
     };
 };
 
+// One row tile: its rows and the steps of positions that some row of it sees.
+struct RowTile {
+    int row0, rows_left, first_row, pos0, pos_low, pos_high, first_step, steps;
+    __device__ RowTile(const AttentionKv4Args &a, const DecodePlan &plan, int number, int rows_per_tile, int step) {
+        const int seq = plan.tiles == 1 ? number : number / plan.tiles, tile = plan.tiles == 1 ? 0 : number - seq * plan.tiles;
+        const int heads = a.n_heads / a.cache.n_kv_heads;
+        const Sequence s(a, seq);
+        row0 = s.row0;
+        pos0 = s.pos0;
+        first_row = tile * rows_per_tile;
+        rows_left = s.rows * heads - first_row;
+        pos_low = s.pos0 + first_row / heads;
+        pos_high = s.pos0 + (first_row + min(rows_left, rows_per_tile) - 1) / heads;
+        const int lo = window_begin(a, pos_low), hi = min(pos_high + 1, position_limit(a));
+        first_step = lo / step;
+        steps = rows_left > 0 && hi > lo ? (hi + step - 1) / step - first_step : 0;
+    }
+};
+
+// Where segments and what joins them lie in the workspace. A segment has the number worker + row tile (unique: from one
+// segment to the next of a line one of the two grows): kRows rows of kDim sums, then their (base, sum).
+struct Segments {
+    float *sums, *bases;
+    int2 *parts;  // of each row tile: first worker, and how many (0: it sees nothing)
+    int per_head;
+    __host__ __device__ Segments(const AttentionKv4Args &a, const DecodePlan &plan, int rows) {
+        const int numbers = a.batch.batch * plan.tiles;
+        per_head = plan.workers + numbers;
+        const size_t all = (size_t)a.cache.n_kv_heads * per_head * rows;
+        sums = (float *)a.workspace;
+        bases = sums + all * a.cache.head_dim;
+        parts = (int2 *)(bases + all * 2);
+    }
+    __host__ __device__ static size_t bytes(const AttentionKv4Args &a, const DecodePlan &plan, int rows) {
+        const size_t numbers = (size_t)a.batch.batch * plan.tiles;
+        return (size_t)a.cache.n_kv_heads * (plan.workers + numbers) * rows * (a.cache.head_dim + 2) * 4 + numbers * 8;
+    }
+};
+
+__device__ __forceinline__ void store_row(const AttentionKv4Args &a, size_t query, int head, int d, float4_t o, float total) {
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // nothing seen: 0
+    const uint2_t packed = {(uint32_t)f2h(o[0] * inv) | (uint32_t)f2h(o[1] * inv) << 16, (uint32_t)f2h(o[2] * inv) | (uint32_t)f2h(o[3] * inv) << 16};
+    *(uint2_t *)(a.output + query * a.output_stride + (size_t)head * a.cache.head_dim + d) = packed;
+}
+
 template <int kDim, int kRows>
-__global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const AttentionKv4Args a, const SplitPlan plan) {
+__global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const AttentionKv4Args a, const DecodePlan plan) {
     using D = Decode<kDim, kRows>;
     constexpr int G = D::kGroups;
     __shared__ __align__(16) unsigned char lds[D::kLds];
@@ -116,162 +170,267 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
     const Kv4Cache &c = a.cache;
     const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int quad = lane >> 4, t16 = lane & 15;
-    const int kv = blockIdx.x % c.n_kv_heads;  // fastest: a kv head's parts and tiles fall on the same XCDs
-    const int part = blockIdx.x / c.n_kv_heads % plan.splits, tile = blockIdx.x / c.n_kv_heads / plan.splits;
-    const int seq = blockIdx.y, heads = a.n_heads / c.n_kv_heads;
+    const int kv = blockIdx.x, worker = blockIdx.y + blockIdx.z * gridDim.y;  // kv fastest: a head's pieces fall on the same XCDs
+    if (worker >= plan.workers) return;
+    const int heads = a.n_heads / c.n_kv_heads, numbers = a.batch.batch * plan.tiles;
 
-    const Sequence s(a, seq);
-    const int first_row = tile * kRows, rows_left = s.rows * heads - first_row;  // rows are (query row, head), heads fastest
-    if (rows_left <= 0) return;
-    const int last_row = first_row + min(rows_left, kRows) - 1;
-    const int pos_low = s.pos0 + first_row / heads, pos_high = s.pos0 + last_row / heads;
-    const Span span(window_begin(a, pos_low), min(pos_high + 1, position_limit(a)), D::kStep, plan.splits);
-    if (plan.splits > 1 && part >= span.used) return;  // (one part: it writes the zeros of rows that see nothing)
-
-    // row operands: this lane's row and its 8 dims of each group
-    // (rows that are not there are zeros; what they see shows in their own columns only)
-    half8_t q[G];
-    float own_sum[G];
-    {
-        const int row = t16 % kRows, at = first_row + row;
-        const bool real = row < rows_left;
-        const uint16_t *src = a.q + (size_t)(s.row0 + (real ? at / heads : 0)) * a.q_stride + (size_t)(kv * heads + (real ? at % heads : 0)) * kDim + quad * 8;
+    // this workgroup's piece of the line, and the row tile that it begins in
+    int number = worker, offset = 0, left = INT32_MAX;
+    if (!plan.alone) {
+        int total = 0;
+        for (int base = 0; base < numbers; base += kWave)
+            total += base + lane < numbers ? RowTile(a, plan, base + lane, kRows, D::kStep).steps : 0;
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            half8_t x = real ? *(const half8_t *)(src + g * 32) : half8_t{};
-            own_sum[g] = 0;
+        for (int off = 1; off < kWave; off <<= 1) total += __shfl_xor(total, off, kWave);
+        const int per = max(plan.least, (total + plan.workers - 1) / plan.workers);
+        const long long begin = (long long)worker * per;
+        const bool scribe = kv == 0 && worker == 0 && wave == 0;
+        left = (int)min((long long)per, total - begin);
+        if (left <= 0 && !(kv == 0 && worker == 0)) return;
+        const Segments segments(a, plan, kRows);
+        int before = 0;
+        number = -1;
+        for (int base = 0; base < numbers && (number < 0 || scribe); base += kWave) {
+            const int steps = base + lane < numbers ? RowTile(a, plan, base + lane, kRows, D::kStep).steps : 0;
+            int upto = steps;
 #pragma unroll
-            for (int j = 0; j < 8; j++) own_sum[g] += (float)x[j];
-            own_sum[g] += __shfl_xor(own_sum[g], 16, kWave);
-            own_sum[g] += __shfl_xor(own_sum[g], 32, kWave);
-            q[g] = x;
-        }
-    }
-    // the four rows that this lane has results of: 4 * row_quad + r
-    const int row_quad = quad % (kRows / 4), pack = quad / (kRows / 4);
-    float q_sum[G][4];
-    int pos[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-#pragma unroll
-        for (int g = 0; g < G; g++) q_sum[g][r] = __shfl(own_sum[g], 4 * quad + r, kWave);
-        const int row = 4 * row_quad + r;
-        pos[r] = row < rows_left ? s.pos0 + (first_row + row) / heads : -1;
-    }
-
-    const size_t code_words = kv4_code_words(1 << c.page_shift, kDim), scale_words = kv4_scale_words(1 << c.page_shift, kDim);
-    const int *table = a.batch.table + (size_t)seq * a.batch.width;
-    const uint32_t key_offset = (uint32_t)(t16 * D::kWords + quad * G);
-    const uint32_t value_offset = (uint32_t)(quad * (D::kWords * 4) + (t16 / D::kLanesPerWord) * 4);
-
-    auto find = [&](int step) {
-        typename D::Places x;
-        const int at = step * D::kStep;
-        x.there = 0;
-#pragma unroll
-        for (int i = 0; i < D::kTiles; i++) {
-            const int index = (at + 16 * i) >> c.page_shift;
-            const int page = index < a.batch.width ? table[index] : -1;
-            const bool there = page >= 0 && page < c.n_pages;
-            x.there |= (uint32_t)there << i;
-            x.block[i] = (there ? page : 0) * c.n_kv_heads + kv;
-            x.slot[i] = (at + 16 * i) & ((1 << c.page_shift) - 1);
-        }
-        return x;
-    };
-    auto load_keys = [&](typename D::Keys &x, const typename D::Places &at) {
-#pragma unroll
-        for (int i = 0; i < D::kTiles; i++)
-            x.k[i] = *(const typename D::KeyWords *)(c.k_codes + (size_t)at.block[i] * code_words + (size_t)at.slot[i] * D::kWords + key_offset);
-#pragma unroll
-        for (int p = 0; p < D::kPasses; p++) {
-            int b = at.block[p * D::kPack], sl = at.slot[p * D::kPack];
-#pragma unroll
-            for (int u = 1; u < D::kPack; u++)
-                if (pack == u) b = at.block[p * D::kPack + u], sl = at.slot[p * D::kPack + u];
-            const size_t word = (size_t)b * scale_words + sl + t16;
-#pragma unroll
-            for (int g = 0; g < G; g++) {
-                x.km[p][g] = c.k_scales[word + ((size_t)g << c.page_shift)];
-                x.vm[p][g] = c.v_scales[word + ((size_t)g << c.page_shift)];
+            for (int off = 1; off < kWave; off <<= 1) {
+                const int v = __shfl_up(upto, off, kWave);
+                upto += lane >= off ? v : 0;
             }
+            const int from = before + upto - steps;
+            if (scribe && base + lane < numbers)
+                segments.parts[base + lane] = make_int2(from / per, steps ? (from + steps - 1) / per - from / per + 1 : 0);
+            const unsigned long long here = __ballot(number < 0 && steps > 0 && begin >= from && begin < from + steps);
+            if (here) {
+                const int l = __ffsll((unsigned long long)here) - 1;
+                number = base + l;
+                offset = (int)begin - __shfl(from, l, kWave);
+            }
+            before += __shfl(upto, kWave - 1, kWave);
         }
-    };
-    auto load_values = [&](typename D::Values &x, const typename D::Places &at) {
-#pragma unroll
-        for (int i = 0; i < D::kTiles; i++)
-#pragma unroll
-            for (int e = 0; e < D::kSets; e++)
-                x.v[i][e] = *(const uint4_t *)(c.v_codes + (size_t)at.block[i] * code_words + (size_t)at.slot[i] * D::kWords + value_offset + e * D::kSetWords * 4);
-    };
+        if (left <= 0) return;  // (nothing at all to see)
+    }
+    number = __builtin_amdgcn_readfirstlane(number);
+    offset = __builtin_amdgcn_readfirstlane(offset);
+    left = __builtin_amdgcn_readfirstlane(left);
 
     const int limit = position_limit(a);
-    float4_t acc[D::kSets][D::kNibbles] = {};
-    float acc_min[G][4] = {}, sum[4] = {}, top[4], base[4];
-#pragma unroll
-    for (int r = 0; r < 4; r++) top[r] = base[r] = kEmpty;
-    int power = -24;            // 2^power is at least every step of the values seen so far
-    uint32_t power_bits = 0;    // ... as fp16 bits (steps are positive: their bits compare as the numbers do)
-    const float c_min = a.scale * 1.44269504088896f, c_even = c_min * 16777216.0f, c_odd = c_min * 1048576.0f;
+    const int row_quad = quad % (kRows / 4), pack = quad / (kRows / 4);  // this lane's results: rows 4 * row_quad + r of tile `pack`
+    const size_t code_words = kv4_code_words(1 << c.page_shift, kDim), scale_words = kv4_scale_words(1 << c.page_shift, kDim);
+    // this lane's bytes in a tile: its position's words of its depth, four positions of its word, its position's step and minimum
+    const uint32_t key_offset = (uint32_t)(t16 * D::kWords + quad * G) * 4;
+    const uint32_t value_offset = (uint32_t)(quad * (D::kWords * 4) + (t16 / D::kLanesPerWord) * 4) * 4;
+    const uint32_t scale_offset = (uint32_t)(16 * pack + t16) * 4;
+    const float sign = t16 & 1 ? -1.0f : 1.0f, flipped = t16 & 1 ? 15.0f : 0.0f;  // of this lane's positions
+    float minus_one = -1.0f;  // (a variable: the product with it is folded into a mixed-precision instruction, a difference is not)
+    asm("" : "+v"(minus_one));
+    const float c_low = a.scale * 1.44269504088896f, c_even = c_low * 16777216.0f, c_odd = c_low * 1048576.0f;
     unsigned char *mine = lds + wave * D::kWaveBytes;
 
-    auto work = [&](const typename D::Keys &x, const typename D::Values &y, uint32_t pages, int step, bool whole) {
-        float raw[D::kPasses][4], most = -INFINITY;
-        uint32_t vm[D::kPasses][G], largest = 0, sees = ~0u;  // sees: bit 4 p + r
+    while (true) {
+        const RowTile tile(a, plan, number, kRows, D::kStep);
+        const int count = min(tile.steps - offset, left);
+        const bool entire = plan.alone || (offset == 0 && count == tile.steps);
+        if (tile.rows_left <= 0) return;  // (alone only)
+        const int *table = a.batch.table + (size_t)(plan.tiles == 1 ? number : number / plan.tiles) * a.batch.width;
+
+        // 64 entries of the page table at a time, one per lane: a step's pages are then a lane read away (a load of their own
+        // would stand in front of every step's loads)
+        int held_from = INT32_MIN, held = -1;
+        auto find = [&](int step) {
+            typename D::Places x;
+            const int at = step * D::kStep, last = (at + 16 * (D::kTiles - 1)) >> c.page_shift;
+            if (held_from == INT32_MIN || last >= held_from + kWave) {
+                held_from = at >> c.page_shift;
+                held = table[min(held_from + lane, a.batch.width - 1)];
+            }
+            x.there = 0;
 #pragma unroll
-        for (int p = 0; p < D::kPasses; p++) {
-            float4_t d[G];
+            for (int i = 0; i < D::kTiles; i++) {
+                const int index = (at + 16 * i) >> c.page_shift;
+                const int page = __builtin_amdgcn_readlane(held, index - held_from);
+                const bool there = index < a.batch.width && page >= 0 && page < c.n_pages;
+                x.there |= (uint32_t)there << i;
+                x.block[i] = (there ? page : 0) * c.n_kv_heads + kv;
+                x.slot[i] = (at + 16 * i) & ((1 << c.page_shift) - 1);
+            }
+            return x;
+        };
+        const bool one_page = 1 << c.page_shift >= D::kStep;  // a step's positions lie in one page
+        const auto bytes = [](const void *at, size_t words) { return (const unsigned char *)at + words * 4; };
+        auto load_keys = [&](typename D::Keys &x, const typename D::Places &at) {
 #pragma unroll
-            for (int pair = 0; pair < G / 2; pair++)
+            for (int i = 0; i < D::kTiles; i++)
+                x.k[i] = *(const typename D::KeyWords *)(bytes(c.k_codes, at.block[i] * code_words + (size_t)at.slot[i] * D::kWords) + key_offset);
+            if (one_page) {
+                const size_t word = at.block[0] * scale_words + at.slot[0];
 #pragma unroll
-                for (int u = 0; u < D::kPack; u++) {
-                    const uint32_t w0 = x.k[p * D::kPack + u][2 * pair], w1 = x.k[p * D::kPack + u][2 * pair + 1];
-                    const uint4_t even = {w0 & kEvenCodes, w0 >> 8 & kEvenCodes, w1 & kEvenCodes, w1 >> 8 & kEvenCodes};
-                    const uint4_t odd = {w0 & kOddCodes, w0 >> 8 & kOddCodes, w1 & kOddCodes, w1 >> 8 & kOddCodes};
-                    const float4_t d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair], __builtin_bit_cast(half8_t, even), float4_t{}, 0, 0, 0);
-                    const float4_t d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair + 1], __builtin_bit_cast(half8_t, odd), float4_t{}, 0, 0, 0);
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int p = 0; p < D::kPasses; p++) {
+                        x.km[p][g] = *(const uint32_t *)(bytes(c.k_scales, word + ((size_t)g << c.page_shift)) + scale_offset + p * D::kPack * 64);
+                        x.vm[p][g] = *(const uint32_t *)(bytes(c.v_scales, word + ((size_t)g << c.page_shift)) + scale_offset + p * D::kPack * 64);
+                    }
+            } else {
+#pragma unroll
+                for (int p = 0; p < D::kPasses; p++) {
+                    uint32_t b = at.block[p * D::kPack], sl = at.slot[p * D::kPack];
+#pragma unroll
+                    for (int u = 1; u < D::kPack; u++)
+                        if (pack == u) b = at.block[p * D::kPack + u], sl = at.slot[p * D::kPack + u];
+                    const size_t word = b * scale_words + sl + t16;
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        x.km[p][g] = c.k_scales[word + ((size_t)g << c.page_shift)];
+                        x.vm[p][g] = c.v_scales[word + ((size_t)g << c.page_shift)];
+                    }
+                }
+            }
+        };
+        auto load_values = [&](typename D::Values &x, const typename D::Places &at) {
+#pragma unroll
+            for (int i = 0; i < D::kTiles; i++)
+#pragma unroll
+                for (int e = 0; e < D::kSets; e++)
+                    x.v[i][e] = *(const uint4_t *)(bytes(c.v_codes, at.block[i] * code_words + (size_t)at.slot[i] * D::kWords + e * D::kSetWords * 4) + value_offset);
+        };
+
+        int step = tile.first_step + offset + wave;
+        const int end = tile.first_step + offset + count;
+        typename D::Places at;
+        typename D::Keys now;
+        if (step < end) {
+            at = find(step);
+            load_keys(now, at);
+        }
+
+        // row operands: this lane's row and its 8 dims of each group; and the groups' sums, which the minima multiply, as one
+        // more operand: first and second fp16 piece of sum / 32 at the depth of the quad that holds the minima of the row's tile
+        // (rows that are not there are zeros; what they see shows in their own columns only)
+        half8_t q[G], q_sums = {};
+        {
+            const int row = t16 % kRows, at_row = tile.first_row + row;
+            const bool real = row < tile.rows_left;
+            const uint16_t *src = a.q + (size_t)(tile.row0 + (real ? at_row / heads : 0)) * a.q_stride + (size_t)(kv * heads + (real ? at_row % heads : 0)) * kDim + quad * 8;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                q[g] = real ? *(const half8_t *)(src + g * 32) : half8_t{};
+                float sum = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) sum += (float)q[g][j];
+                sum += __shfl_xor(sum, 16, kWave);
+                sum += __shfl_xor(sum, 32, kWave);
+                sum *= 0.03125f;
+                if (quad == t16 / kRows * (kRows / 4)) {
+                    q_sums[g] = (_Float16)sum;
+                    q_sums[G + g] = (_Float16)(sum - (float)q_sums[g]);
+                }
+            }
+        }
+
+        float4_t acc[D::kSets][D::kNibbles] = {};
+        float acc_min[G][4] = {}, sum[4] = {}, base[4] = {kEmpty, kEmpty, kEmpty, kEmpty};
+        int power = -24;          // 2^power is at least every step of the values seen so far
+        uint32_t power_bits = 0;  // ... as fp16 bits (steps are positive: their bits compare as the numbers do)
+
+        // this step's values, which the work on the scores covers, then the next step's keys
+        while (step < end) {
+            typename D::Values values;
+            load_values(values, at);
+            const uint32_t pages = at.there;
+            const int first = step * D::kStep;
+            typename D::Keys next;
+            step += kWaves;
+            if (step < end) {
+                at = find(step);
+                load_keys(next, at);
+            }
+            // whole: every row sees all of the step's positions
+            const bool whole = pages == (1u << D::kTiles) - 1 && first + D::kStep - 1 <= tile.pos_low && first + D::kStep <= limit &&
+                               (a.window == 0 || first > tile.pos_high - a.window);
+            float raw[D::kPasses][4], most = -INFINITY;
+            uint32_t largest = 0, sees = ~0u;  // sees: bit 4 p + r
+#pragma unroll
+            for (int p = 0; p < D::kPasses; p++) {
+                float4_t d[G];
+#pragma unroll
+                for (int pair = 0; pair < G / 2; pair++)
+#pragma unroll
+                    for (int u = 0; u < D::kPack; u++) {
+                        const uint32_t w0 = now.k[p * D::kPack + u][2 * pair], w1 = now.k[p * D::kPack + u][2 * pair + 1];
+                        const uint4_t even = {w0 & kEvenCodes, w0 >> 8 & kEvenCodes, w1 & kEvenCodes, w1 >> 8 & kEvenCodes};
+                        const uint4_t odd = {w0 & kOddCodes, w0 >> 8 & kOddCodes, w1 & kOddCodes, w1 >> 8 & kOddCodes};
+                        const float4_t d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair], __builtin_bit_cast(half8_t, even), float4_t{}, 0, 0, 0);
+                        const float4_t d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair + 1], __builtin_bit_cast(half8_t, odd), float4_t{}, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            d[2 * pair][r] = u == 0 || pack == u ? d0[r] : d[2 * pair][r];
+                            d[2 * pair + 1][r] = u == 0 || pack == u ? d1[r] : d[2 * pair + 1][r];
+                        }
+                        if (u & 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                bool unsound = false;
+                if (!whole) {
+                    asm volatile("");  // (a branch: not worked out and chosen from in every step)
+                    const int t = first + 16 * (p * D::kPack + pack) + t16;
+                    const bool there = (pages >> (p * D::kPack + pack) & 1) && t < limit;
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        d[2 * pair][r] = u == 0 || pack == u ? d0[r] : d[2 * pair][r];
-                        d[2 * pair + 1][r] = u == 0 || pack == u ? d1[r] : d[2 * pair + 1][r];
+                        const int row = 4 * row_quad + r, pos = tile.pos0 + (tile.first_row + row) / heads;
+                        const bool one = there && row < tile.rows_left && t <= pos && (a.window == 0 || t > pos - a.window);
+                        sees &= ~((uint32_t)!one << (4 * p + r));
                     }
-                    if (u & 1) __builtin_amdgcn_sched_barrier(0);
-                }
+                    // What no row sees may be anything, and must reach neither the powers below nor, in the product of the
+                    // minima, the other tiles' positions. Nor must what is not finite and only some rows see reach the others:
+                    // a key's rows get their NaN in the scores below, a value's in the sum of its group's minima.
+                    const bool any = there && t <= tile.pos_high && (a.window == 0 || t > tile.pos_low - a.window);
 #pragma unroll
-            for (int g = 0; g < G; g++) vm[p][g] = x.vm[p][g];
-            if (!whole) {
-                const int at = step * D::kStep + 16 * (p * D::kPack + pack) + t16;
-                const bool there = (pages >> (p * D::kPack + pack) & 1) && at < limit;
+                    for (int g = 0; g < G; g++) {
+                        unsound |= any && (now.km[p][g] & 0x7C000000u) == 0x7C000000u;
+                        const bool wrong = any && ((now.vm[p][g] & 0x7C000000u) == 0x7C000000u || (now.vm[p][g] & 0x7C00u) == 0x7C00u);
+                        now.vm[p][g] = any && !wrong ? now.vm[p][g] : 0;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc_min[g][r] = wrong && (sees >> (4 * p + r) & 1) ? NAN : acc_min[g][r];
+                    }
+#pragma unroll
+                    for (int g = 0; g < G; g++) now.km[p][g] = any && !unsound ? now.km[p][g] : 0;
+                }
+                uint4_t minima;
+#pragma unroll
+                for (int j = 0; j < 4; j++)  // (G is 2: the last four depths have zero rows, and zeros here)
+                    minima[j] = G == 4 || j < 2 ? __builtin_amdgcn_perm(now.km[p][2 * j % G + 1], now.km[p][2 * j % G], 0x07060302u) : 0;
+                const float4_t low = __builtin_amdgcn_mfma_f32_16x16x32_f16(q_sums, __builtin_bit_cast(half8_t, minima), float4_t{}, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const bool one = there && at <= pos[r] && (a.window == 0 || at > pos[r] - a.window);
-                    sees &= ~((uint32_t)!one << (4 * p + r));
+                    float even = 0, odd = 0;
+#pragma unroll
+                    for (int g = 0; g < G; g += 2) {
+                        even = __builtin_fmaf(low_half(now.km[p][g]), d[g][r], even);
+                        odd = __builtin_fmaf(low_half(now.km[p][g + 1]), d[g + 1][r], odd);
+                    }
+                    raw[p][r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low[r] * (32.0f * c_low)));
+                }
+                if (!whole) {
+                    asm volatile("");
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        raw[p][r] = unsound ? NAN : raw[p][r];
+                        raw[p][r] = sees >> (4 * p + r) & 1 ? raw[p][r] : -INFINITY;
+                    }
                 }
 #pragma unroll
-                for (int g = 0; g < G; g++) vm[p][g] = sees >> (4 * p) & 15 ? vm[p][g] : 0;  // what lies there must not reach the powers below
+                for (int r = 0; r < 4; r++) most = fmaxf(most, raw[p][r] - base[r]);
+#pragma unroll
+                for (int g = 0; g < G; g++) largest = max(largest, now.vm[p][g] & 0xFFFFu);
             }
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float even = 0, odd = 0, low = 0;
-#pragma unroll
-                for (int g = 0; g < G; g++) {
-                    if (g & 1) odd = __builtin_fmaf(low_half(x.km[p][g]), d[g][r], odd);
-                    else even = __builtin_fmaf(low_half(x.km[p][g]), d[g][r], even);
-                    low = __builtin_fmaf(high_half(x.km[p][g]), q_sum[g][r], low);
-                }
-                raw[p][r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low * c_min));
-                raw[p][r] = sees >> (4 * p + r) & 1 ? raw[p][r] : -INFINITY;
-                most = fmaxf(most, raw[p][r] - base[r]);
-            }
-#pragma unroll
-            for (int g = 0; g < G; g++) largest = max(largest, vm[p][g] & 0xFFFFu);
-        }
-        const bool grown = most > (float)(kHeadroom + kTopPower - power) || largest > power_bits;
+            const bool grown = most > (float)(kHeadroom + kTopPower - power) || largest > power_bits;
             if (__ballot(grown)) {
                 // rare after the first steps: new bases (a base is the row's largest score so far, moved by the powers)
                 int bits = (int)largest;
 #pragma unroll
                 for (int off = 1; off < kWave; off <<= 1) bits = max(bits, __shfl_xor(bits, off, kWave));
+                const float moved = (float)(power - kTopPower);
                 if ((uint32_t)bits > power_bits) {
                     if (bits > 0x7BFF) bits = 0x7BFF;  // (infinite or NaN: the weights carry it on)
                     int e;
@@ -285,14 +444,12 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
                     float m = raw[0][r];
 #pragma unroll
                     for (int p = 1; p < D::kPasses; p++) m = fmaxf(m, raw[p][r]);
-#pragma unroll
-                    for (int off = 1; off < 16; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
+                    m = quad_max(m);
 #pragma unroll
                     for (int off = 4 * kRows; off < kWave; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
-                    top[r] = fmaxf(top[r], m);
-                    const float now = top[r] + (float)(power - kTopPower);
-                    keep[r] = __builtin_amdgcn_exp2f(base[r] - now);
-                    base[r] = now;
+                    const float to = fmaxf(base[r] - moved, m) + (float)(power - kTopPower);
+                    keep[r] = __builtin_amdgcn_exp2f(base[r] - to);
+                    base[r] = to;
                     sum[r] *= keep[r];
 #pragma unroll
                     for (int g = 0; g < G; g++) acc_min[g][r] *= keep[r];
@@ -310,229 +467,198 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
                     for (int i = 0; i < D::kNibbles; i++) acc[e][i] *= column;
             }
 #pragma unroll
-        for (int p = 0; p < D::kPasses; p++) {
-            float w[4];
+            for (int p = 0; p < D::kPasses; p++) {
+                float w[4];
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                w[r] = __builtin_amdgcn_exp2f(raw[p][r] - base[r]);
-                sum[r] += w[r];
-            }
-            unsigned char *at = mine + (16 * (p * D::kPack + pack) + t16) * D::kRowBytes + row_quad * 8;
-            auto weigh = [&](auto keep) {
+                for (int r = 0; r < 4; r++) {
+                    w[r] = __builtin_amdgcn_exp2f(raw[p][r] - base[r]);
+                    sum[r] += w[r];
+                }
+                unsigned char *to = mine + (16 * (p * D::kPack + pack) + t16) * D::kRowBytes + row_quad * 8;
 #pragma unroll
                 for (int g = 0; g < G; g++) {
-                    const float low = __builtin_fmaf(low_half(vm[p][g]), 8.0f, high_half(vm[p][g]));  // of code 8
+                    const float size = low_half(now.vm[p][g]) * sign, low = __builtin_fmaf(low_half(now.vm[p][g]), flipped, high_half(now.vm[p][g]));
                     float ws[4];
                     uint32_t hi[2], lo[2];
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        ws[r] = keep(r, w[r] * low_half(vm[p][g]), 0.0f);
-                        acc_min[g][r] = keep(r, __builtin_fmaf(w[r], low, acc_min[g][r]), acc_min[g][r]);
+                        ws[r] = w[r] * size;
+                        acc_min[g][r] = __builtin_fmaf(w[r], low, acc_min[g][r]);
                     }
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        // (both to nearest: the codes are all positive, so a bias of 2^-22 would add up over a long context
-                        // to more than what is left of the values' average, 2^-22 * 2 sqrt(positions))
                         const half2_t h = {(_Float16)ws[2 * j], (_Float16)ws[2 * j + 1]};
-                        const half2_t l = {(_Float16)(ws[2 * j] - (float)h[0]), (_Float16)(ws[2 * j + 1] - (float)h[1])};
+                        const half2_t l = {(_Float16)__builtin_fmaf((float)h[0], minus_one, ws[2 * j]), (_Float16)__builtin_fmaf((float)h[1], minus_one, ws[2 * j + 1])};
                         hi[j] = __builtin_bit_cast(uint32_t, h);
                         lo[j] = __builtin_bit_cast(uint32_t, l);
                     }
-                    *(uint2_t *)(at + g * kRows * 2) = uint2_t{hi[0], hi[1]};
-                    *(uint2_t *)(at + D::kColumns * 2 + g * kRows * 2) = uint2_t{lo[0], lo[1]};
+                    *(uint2_t *)(to + g * kRows * 2) = uint2_t{hi[0], hi[1]};
+                    *(uint2_t *)(to + D::kColumns * 2 + g * kRows * 2) = uint2_t{lo[0], lo[1]};
                 }
-            };
-            // (what a row does not see may be anything, NaN too, also where another row sees it: taken out by choice, not by a zero)
-            if (whole) weigh([](int, float x, float) { return x; });
-            else weigh([&](int r, float x, float other) { return sees >> (4 * p + r) & 1 ? x : other; });
-        }
-        // (the lanes read each other's weights: the wave's LDS accesses run in order, the compiler has to keep it)
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+            }
+            // (the lanes read each other's weights: the wave's LDS accesses run in order, the compiler has to keep it)
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int half = 0; half < D::kTiles / 2; half++) {
-            half8_t weights[D::kSets][2];
+            for (int half = 0; half < D::kTiles / 2; half++) {
+                half8_t weights[D::kSets][2];
 #pragma unroll
-            for (int e = 0; e < D::kSets; e++)
+                for (int e = 0; e < D::kSets; e++)
 #pragma unroll
-                for (int piece = 0; piece < 2; piece++) {
-                    short4_t two[2];
+                    for (int piece = 0; piece < 2; piece++) {
+                        short4_t two[2];
 #pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        unsigned char *from = mine + (16 * (2 * half + i) + 4 * quad + (lane >> 2 & 3)) * D::kRowBytes + piece * D::kColumns * 2 + e * 32 + (lane & 3) * 8;
-                        two[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)from);
-                    }
-                    struct Both { short4_t x[2]; } both = {{two[0], two[1]}};
-                    weights[e][piece] = __builtin_bit_cast(half8_t, both);
-                }
-#pragma unroll
-            for (int e = 0; e < D::kSets; e++) {
-                const uint4_t va = y.v[2 * half][e], vb = y.v[2 * half + 1][e];
-                constexpr int kPieces = D::kNibbles == 8 ? 2 : 1;
-#pragma unroll
-                for (int piece = 0; piece < kPieces; piece++) {
-                    // one 16-bit piece of two positions' words side by side (a byte where four lanes share a word)
-                    uint32_t select;
-                    if constexpr (D::kNibbles == 8) select = piece ? 0x07060302u : 0x05040100u;
-                    else if constexpr (D::kNibbles == 4) select = t16 & 1 ? 0x07060302u : 0x05040100u;
-                    else select = 0x0C000C00u | (uint32_t)((t16 & 3) + 4) << 16 | (uint32_t)(t16 & 3);
-                    const uint32_t pairs[4] = {__builtin_amdgcn_perm(va[1], va[0], select), __builtin_amdgcn_perm(va[3], va[2], select),
-                                               __builtin_amdgcn_perm(vb[1], vb[0], select), __builtin_amdgcn_perm(vb[3], vb[2], select)};
-#pragma unroll
-                    for (int i = 0; i < (D::kNibbles < 4 ? D::kNibbles : 4); i++) {
-                        half8_t codes;
-#pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            const uint32_t field = i & 2 ? pairs[j] >> 8 : pairs[j];
-                            const half2_t two = __builtin_bit_cast(half2_t, i & 1 ? (field & kOddCodes) | kOddBits : (field & kEvenCodes) | kEvenBits) -
-                                                (i & 1 ? half2_t{72, 72} : half2_t{1032, 1032});
-                            codes[2 * j] = two[0];
-                            codes[2 * j + 1] = two[1];
+                        for (int i = 0; i < 2; i++) {
+                            unsigned char *from = mine + (16 * (2 * half + i) + 4 * quad + (lane >> 2 & 3)) * D::kRowBytes + piece * D::kColumns * 2 + e * 32 + (lane & 3) * 8;
+                            two[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)from);
                         }
-                        float4_t &into = acc[e][piece * 4 + i];
-                        into = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, weights[e][0], into, 0, 0, 0);
-                        into = __builtin_amdgcn_mfma_f32_16x16x32_f16(codes, weights[e][1], into, 0, 0, 0);
-                        if (i & 1) __builtin_amdgcn_sched_barrier(0);
+                        struct Both { short4_t x[2]; } both = {{two[0], two[1]}};
+                        weights[e][piece] = __builtin_bit_cast(half8_t, both);
+                    }
+#pragma unroll
+                for (int e = 0; e < D::kSets; e++) {
+                    const uint4_t va = values.v[2 * half][e], vb = values.v[2 * half + 1][e];
+#pragma unroll
+                    for (int byte = 0; byte < D::kNibbles / 2; byte++) {
+                        // this lane's byte `byte` of two positions' words, one per half
+                        const uint32_t which = (uint32_t)(t16 % D::kLanesPerWord * (D::kNibbles / 2) + byte), select = which * 0x00010001u + 0x0C040C00u;
+                        const uint32_t pairs[4] = {__builtin_amdgcn_perm(va[1], va[0], select), __builtin_amdgcn_perm(va[3], va[2], select),
+                                                   __builtin_amdgcn_perm(vb[1], vb[0], select), __builtin_amdgcn_perm(vb[3], vb[2], select)};
+#pragma unroll
+                        for (int odd = 0; odd < 2; odd++) {
+                            uint4_t codes;
+#pragma unroll
+                            for (int j = 0; j < 4; j++) codes[j] = ((odd ? pairs[j] : pairs[j] << 4) ^ kSecondFlipped) & kOddCodes;
+                            float4_t &into = acc[e][2 * byte + odd];
+                            into = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes), weights[e][0], into, 0, 0, 0);
+                            into = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes), weights[e][1], into, 0, 0, 0);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            now = next;
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    };
 
-    const int end = min(span.first + span.steps, span.first + (part + 1) * span.per);
-    int step = span.first + part * span.per + wave;
-    for (; step < end; step += kWaves) {
-        const typename D::Places at = find(step);
-        typename D::Keys keys;
-        typename D::Values values;
-        load_keys(keys, at);
-        load_values(values, at);
-        const int first = step * D::kStep;
-        const bool whole = at.there == (1u << D::kTiles) - 1 && first + D::kStep - 1 <= pos_low && first + D::kStep <= limit &&
-                           (a.window == 0 || first > pos_high - a.window);
-        work(keys, values, at.there, step, whole);
-    }
-
-    // ---- the wave's sums over its lanes
-#pragma unroll
-    for (int r = 0; r < 4; r++) {
-#pragma unroll
-        for (int off = 1; off < 16; off <<= 1) {
-            sum[r] += __shfl_xor(sum[r], off, kWave);
-#pragma unroll
-            for (int g = 0; g < G; g++) acc_min[g][r] += __shfl_xor(acc_min[g][r], off, kWave);
-        }
-#pragma unroll
-        for (int off = 4 * kRows; off < kWave; off <<= 1) {
-            sum[r] += __shfl_xor(sum[r], off, kWave);
-#pragma unroll
-            for (int g = 0; g < G; g++) acc_min[g][r] += __shfl_xor(acc_min[g][r], off, kWave);
-        }
-    }
-    if (t16 == 0 && pack == 0) {
+        // ---- the wave's sums over its lanes
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            join_base[wave][4 * row_quad + r] = base[r];
-            join_sum[wave][4 * row_quad + r] = sum[r];
+            sum[r] = quad_sum(sum[r]);
+#pragma unroll
+            for (int g = 0; g < G; g++) acc_min[g][r] = quad_sum(acc_min[g][r]);
+#pragma unroll
+            for (int off = 4 * kRows; off < kWave; off <<= 1) {
+                sum[r] += __shfl_xor(sum[r], off, kWave);
+#pragma unroll
+                for (int g = 0; g < G; g++) acc_min[g][r] += __shfl_xor(acc_min[g][r], off, kWave);
+            }
         }
-    }
-    // this lane's column is (group in the set, row): the minima's share of each set's group
-    const int row = t16 % kRows, in_set = t16 / kRows;
-    float low[D::kSets];
-#pragma unroll
-    for (int e = 0; e < D::kSets; e++) {
-        low[e] = 0;
-#pragma unroll
-        for (int g = 0; g < D::kSetGroups; g++)
+        if (t16 == 0 && pack == 0) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float v = __shfl(acc_min[e * D::kSetGroups + g][r], (row >> 2) * 16, kWave);
-                if (in_set == g && (row & 3) == r) low[e] = v;
+                join_base[wave][4 * row_quad + r] = base[r];
+                join_sum[wave][4 * row_quad + r] = sum[r];
             }
-    }
-    __syncthreads();  // (also: every wave is through with its weights in LDS)
-    float highest = kEmpty;
+        }
+        // this lane's column is (group in the set, row): the minima's share of each set's group
+        const int row = t16 % kRows, in_set = t16 / kRows;
+        float low[D::kSets];
 #pragma unroll
-    for (int w = 0; w < kWaves; w++) highest = fmaxf(highest, join_base[w][row]);
-    const float mine_keep = __builtin_amdgcn_exp2f(join_base[wave][row] - highest);
-    float *out = (float *)lds + (size_t)wave * kRows * kDim + row * kDim;
+        for (int e = 0; e < D::kSets; e++) {
+            low[e] = 0;
 #pragma unroll
-    for (int e = 0; e < D::kSets; e++)
+            for (int g = 0; g < D::kSetGroups; g++)
 #pragma unroll
-        for (int i = 0; i < D::kNibbles; i++)
+                for (int r = 0; r < 4; r++) {
+                    const float v = __shfl(acc_min[e * D::kSetGroups + g][r], (row >> 2) * 16, kWave);
+                    if (in_set == g && (row & 3) == r) low[e] = v;
+                }
+        }
+        __syncthreads();  // (also: every wave is through with its weights in LDS)
+        float highest = kEmpty;
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int n = 4 * quad + r;  // the operand's row: word n / kLanesPerWord of the set, nibble part n % kLanesPerWord
-                const int dim = (e * D::kSetWords + n / D::kLanesPerWord) * 8 + n % D::kLanesPerWord * D::kNibbles + i;
-                const float v = acc[e][i][r] + low[e];
-                if (in_set < D::kSetGroups && dim / 32 - e * D::kSetGroups == in_set) out[dim] = v * mine_keep;
+        for (int w = 0; w < kWaves; w++) highest = fmaxf(highest, join_base[w][row]);
+        const float mine_keep = __builtin_amdgcn_exp2f(join_base[wave][row] - highest);
+        float *out = (float *)lds + (size_t)wave * kRows * kDim + row * kDim;
+#pragma unroll
+        for (int e = 0; e < D::kSets; e++)
+#pragma unroll
+            for (int i = 0; i < D::kNibbles; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int n = 4 * quad + r;  // the operand's row: word n / kLanesPerWord of the set, nibble part n % kLanesPerWord
+                    const int dim = (e * D::kSetWords + n / D::kLanesPerWord) * 8 + n % D::kLanesPerWord * D::kNibbles + i;
+                    if (in_set < D::kSetGroups && dim / 32 - e * D::kSetGroups == in_set) out[dim] = __builtin_fmaf(acc[e][i][r], 1048576.0f, low[e]) * mine_keep;
+                }
+        __syncthreads();
+        constexpr int kParts = kDim / 4;  // float4s of a row
+        for (int j = threadIdx.x; j < kRows * kParts; j += kThreads) {
+            const int r = j / kParts, d = j % kParts * 4;
+            if (r >= tile.rows_left) break;
+            float4_t o = {};
+            float m = kEmpty, total = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; w++) {
+                o += *(const float4_t *)((const float *)lds + (size_t)w * kRows * kDim + r * kDim + d);
+                m = fmaxf(m, join_base[w][r]);
             }
-    __syncthreads();
-    constexpr int kParts = kDim / 4;  // float4s of a row
-    for (int j = threadIdx.x; j < kRows * kParts; j += kThreads) {
-        const int r = j / kParts, d = j % kParts * 4;
-        if (r >= rows_left) break;
-        float4_t o = {};
-        float m = kEmpty, total = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-            o += *(const float4_t *)((const float *)lds + (size_t)w * kRows * kDim + r * kDim + d);
-            m = fmaxf(m, join_base[w][r]);
+            for (int w = 0; w < kWaves; w++) total += join_sum[w][r] * __builtin_amdgcn_exp2f(join_base[w][r] - m);
+            if (entire) {
+                const int at_row = tile.first_row + r;
+                store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d, o, total);
+            } else {
+                const Segments segments(a, plan, kRows);
+                const size_t slot = ((size_t)kv * segments.per_head + worker + number) * kRows + r;
+                if (d == 0) *(float2 *)(segments.bases + slot * 2) = make_float2(m, total);
+                *(float4_t *)(segments.sums + slot * kDim + d) = o;
+            }
         }
-#pragma unroll
-        for (int w = 0; w < kWaves; w++) total += join_sum[w][r] * __builtin_amdgcn_exp2f(join_base[w][r] - m);
-        const int at = first_row + r;
-        const size_t query = (size_t)(s.row0 + at / heads);
-        const int head = kv * heads + at % heads;
-        if (plan.splits == 1) {
-            const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // nothing seen: 0
-            const uint2_t packed = {(uint32_t)f2h(o[0] * inv) | (uint32_t)f2h(o[1] * inv) << 16, (uint32_t)f2h(o[2] * inv) | (uint32_t)f2h(o[3] * inv) << 16};
-            *(uint2_t *)(a.output + query * a.output_stride + (size_t)head * kDim + d) = packed;
-        } else {
-            const size_t slot = (query * a.n_heads + head) * plan.splits + part;
-            float *base_sum = (float *)a.workspace + (size_t)a.batch.n_tokens * a.n_heads * plan.splits * kDim + slot * 2;
-            if (d == 0) base_sum[0] = m, base_sum[1] = total;
-            *(float4_t *)((float *)a.workspace + slot * kDim + d) = o;
-        }
+        left -= count;
+        if (plan.alone || left <= 0) return;
+        offset = 0;
+        do {
+            if (++number >= numbers) return;
+        } while (RowTile(a, plan, number, kRows, D::kStep).steps == 0);
+        __syncthreads();
     }
 }
 
-// Joins the parts of one (query row, head): a workgroup each, 16 bytes per lane, kDim / 4 lanes per part.
-template <int kDim>
-__global__ __launch_bounds__(kThreads) void attention_join_kernel(const AttentionKv4Args a, const SplitPlan plan, int rows_per_tile, int step) {
-    constexpr int kLanes = kDim / 4, kAtOnce = kThreads / kLanes;
-    __shared__ float weight[kMostSplits];
-    __shared__ float4_t sums[kAtOnce][kLanes];
-    const int row = blockIdx.x, head = blockIdx.y;
-    const int seq = kv4_find_sequence(a.batch.starts, a.batch.batch, row);
-    if (seq >= a.batch.batch) return;
-    const Sequence s(a, seq);
-    const int i = row - s.row0;
-    if (i < 0 || i >= s.rows) return;
+// Joins the segments of four rows of a row tile; writes the zeros of rows that see nothing. kDim / 4 lanes a row, the
+// segments dealt to kAtOnce groups of lanes, so that a long row's are read in few round trips.
+constexpr int kJoinThreads = 512;
+template <int kDim, int kRows>
+__global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttentionKv4Args a, const DecodePlan plan) {
+    constexpr int kLanes = kDim / 4, kAtOnce = kJoinThreads / (4 * kLanes);
+    __shared__ float4_t sums[kAtOnce][4][kLanes];
+    const int number = blockIdx.x, kv = blockIdx.y;
+    const Segments segments(a, plan, kRows);
+    const int2 parts = segments.parts[number];
+    if (parts.y == 1) return;  // stored at once
+    const RowTile tile(a, plan, number, kRows, Decode<kDim, kRows>::kStep);
+    const int d = threadIdx.x % kLanes, r = blockIdx.z * 4 + threadIdx.x / kLanes % 4, group = threadIdx.x / (4 * kLanes);
     const int heads = a.n_heads / a.cache.n_kv_heads;
-    const int first_row = (i * heads + head % heads) / rows_per_tile * rows_per_tile, last_row = min(first_row + rows_per_tile, s.rows * heads) - 1;
-    const Span span(window_begin(a, s.pos0 + first_row / heads), min(s.pos0 + last_row / heads + 1, position_limit(a)), step, plan.splits);
-    const size_t slot = ((size_t)row * a.n_heads + head) * plan.splits;
-    const float *base_sum = (const float *)a.workspace + (size_t)a.batch.n_tokens * a.n_heads * plan.splits * kDim + slot * 2;
+    if ((int)blockIdx.z * 4 >= tile.rows_left) return;
     float m = kEmpty, total = 0;
-    for (int p = 0; p < span.used; p++) m = fmaxf(m, base_sum[2 * p]);
-    for (int p = 0; p < span.used; p++) total += base_sum[2 * p + 1] * __builtin_amdgcn_exp2f(base_sum[2 * p] - m);
-    if (threadIdx.x < span.used) weight[threadIdx.x] = __builtin_amdgcn_exp2f(base_sum[2 * threadIdx.x] - m);
-    __syncthreads();
-    const int at = threadIdx.x / kLanes, d = threadIdx.x % kLanes;
-    const float4_t *parts = (const float4_t *)((const float *)a.workspace + slot * kDim);
+    const size_t slot = ((size_t)kv * segments.per_head + parts.x + number) * kRows + r;
+    const float2 *bases = (const float2 *)segments.bases + slot;
+#pragma unroll 8
+    for (int p = 0; p < parts.y; p++) m = fmaxf(m, bases[(size_t)p * kRows].x);
+#pragma unroll 8
+    for (int p = 0; p < parts.y; p++) total += bases[(size_t)p * kRows].y * __builtin_amdgcn_exp2f(bases[(size_t)p * kRows].x - m);
+    const float4_t *from = (const float4_t *)(segments.sums + slot * kDim) + d;
     float4_t o = {};
-    for (int p = at; p < span.used; p += kAtOnce) o += parts[(size_t)p * kLanes + d] * weight[p];
-    sums[at][d] = o;
+#pragma unroll 8
+    for (int p = group; p < parts.y; p += kAtOnce) o += from[(size_t)p * kRows * kLanes] * __builtin_amdgcn_exp2f(bases[(size_t)p * kRows].x - m);
+    sums[group][r & 3][d] = o;
     __syncthreads();
-    if (at) return;
+    if (group || r >= tile.rows_left) return;
 #pragma unroll
-    for (int j = 1; j < kAtOnce; j++) o += sums[j][d];
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    const uint2_t packed = {(uint32_t)f2h(o[0] * inv) | (uint32_t)f2h(o[1] * inv) << 16, (uint32_t)f2h(o[2] * inv) | (uint32_t)f2h(o[3] * inv) << 16};
-    *(uint2_t *)(a.output + (size_t)row * a.output_stride + (size_t)head * kDim + d * 4) = packed;
+    for (int j = 1; j < kAtOnce; j++) o += sums[j][r & 3][d];
+    const int at_row = tile.first_row + r;
+    store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d * 4, o, total);
 }
 
 int decode_rows(const AttentionKv4Args &a) {
@@ -540,41 +666,48 @@ int decode_rows(const AttentionKv4Args &a) {
     return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
 }
 
-SplitPlan decode_plan(const AttentionKv4Args &a) {
-    const int rows = decode_rows(a), step = rows == 16 ? 32 : 64;
+DecodePlan decode_plan(const AttentionKv4Args &a) {
+    const int rows = decode_rows(a), step = rows == 4 ? 64 : 32;
     const long long heads = a.n_heads / a.cache.n_kv_heads;
-    SplitPlan p;
-    p.row_tiles = (int)((a.max_query * heads + rows - 1) / rows);
-    long long reach = a.max_length;
-    if (a.window > 0 && (long long)a.window + a.max_query + step < reach) reach = (long long)a.window + a.max_query + step;
-    const long long groups = (long long)p.row_tiles * a.cache.n_kv_heads * a.batch.batch;
-    const long long want = (4ll * current_device_cus() + groups - 1) / groups, most = (reach + kWaves * step - 1) / (kWaves * step);
-    long long n = want < most ? want : most;
-    p.splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    DecodePlan p;
+    p.tiles = (int)((a.max_query * heads + rows - 1) / rows);
+    p.least = 2 * kWaves;
+    long long reach = a.max_length;  // positions that a row tile may see, and the steps that they may touch
+    if (a.window > 0 && (long long)a.window + a.max_query < reach) reach = (long long)a.window + a.max_query;
+    const long long steps = (reach + step - 1) / step + 1;
+    p.alone = steps <= 4 * kWaves;
+    const int slots = 2 * current_device_cus();
+    p.workers = p.alone ? a.batch.batch * p.tiles : (slots + a.cache.n_kv_heads - 1) / a.cache.n_kv_heads;
     return p;
+}
+
+template <int kDim, int kRows>
+hipError_t launch_decode_rows(const AttentionKv4Args &a, const DecodePlan &plan, hipStream_t s) {
+    const int across = plan.workers < 32768 ? plan.workers : 32768;
+    attention_decode_kernel<kDim, kRows><<<dim3((unsigned)a.cache.n_kv_heads, (unsigned)across, (unsigned)((plan.workers + across - 1) / across)), kThreads, 0, s>>>(a, plan);
+    if (!plan.alone) {
+        const dim3 grid((unsigned)(a.batch.batch * plan.tiles), (unsigned)a.cache.n_kv_heads, kRows / 4);
+        if (hipError_t e = hipGetLastError()) return e;
+        attention_join_kernel<kDim, kRows><<<grid, kJoinThreads, 0, s>>>(a, plan);
+    }
+    return hipGetLastError();
 }
 
 template <int kDim>
 hipError_t launch_decode(const AttentionKv4Args &a, hipStream_t s) {
-    const SplitPlan plan = decode_plan(a);
-    const int rows = decode_rows(a);
-    const dim3 grid((unsigned)(a.cache.n_kv_heads * plan.splits) * (unsigned)plan.row_tiles, (unsigned)a.batch.batch);
-    if (rows == 4) attention_decode_kernel<kDim, 4><<<grid, kThreads, 0, s>>>(a, plan);
-    else if (rows == 8) attention_decode_kernel<kDim, 8><<<grid, kThreads, 0, s>>>(a, plan);
-    else attention_decode_kernel<kDim, 16><<<grid, kThreads, 0, s>>>(a, plan);
-    if (hipError_t e = hipGetLastError()) return e;
-    if (plan.splits > 1) {
-        attention_join_kernel<kDim><<<dim3((unsigned)a.batch.n_tokens, (unsigned)a.n_heads), kThreads, 0, s>>>(a, plan, rows, rows == 16 ? 32 : 64);
-        return hipGetLastError();
+    const DecodePlan plan = decode_plan(a);
+    switch (decode_rows(a)) {
+        case 4: return launch_decode_rows<kDim, 4>(a, plan, s);
+        case 8: return launch_decode_rows<kDim, 8>(a, plan, s);
+        default: return launch_decode_rows<kDim, 16>(a, plan, s);
     }
-    return hipSuccess;
 }
 
 }  // namespace
 
 size_t attention_kv4_workspace(const AttentionKv4Args &a) {
-    const SplitPlan plan = decode_plan(a);
-    return plan.splits == 1 ? 0 : (size_t)a.batch.n_tokens * a.n_heads * plan.splits * (a.cache.head_dim + 2) * 4;
+    const DecodePlan plan = decode_plan(a);
+    return plan.alone ? 0 : Segments::bytes(a, plan, decode_rows(a));
 }
 
 hipError_t launch_attention_kv4(const AttentionKv4Args &a, hipStream_t s) {
