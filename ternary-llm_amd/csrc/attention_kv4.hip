@@ -8,6 +8,8 @@
 // same holds for the values: sum_t p_t (m_tg + s_tg c_td) = sum_t (p_t s_tg) c_td + sum_t p_t m_tg with bare codes as one
 // operand and p s as the other. p s is taken in two fp16 pieces (the second is what the first's rounding left), so the only
 // roundings to fewer than 32 bits are 2^-22 of p s, and the result's.
+#include <algorithm>
+
 #include "kv4.h"
 
 namespace tllm {
@@ -20,7 +22,6 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 
-constexpr int kWaves = 4, kThreads = kWaves * kWave;
 constexpr float kEmpty = -1e30f;  // below every score (|q.k| < 2^40, |scale| <= 2^40): no position yet
 constexpr int kHeadroom = 6;      // powers of two that a weight may outgrow its base by before everything is rescaled
 constexpr int kTopPower = 8;      // a base puts the largest weight seen (times its step) at 2^kTopPower
@@ -45,6 +46,19 @@ __device__ __forceinline__ float quad_sum(float v) {
     v += rotated<4>(v);
     v += rotated<2>(v);
     return v + rotated<1>(v);
+}
+// Sum over the lanes up to and including this one.
+template <int kControl, int kRows>
+__device__ __forceinline__ int shifted(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, kControl, kRows, 0xF, false);
+}
+__device__ __forceinline__ int running_sum(int v) {
+    v += shifted<0x111, 0xF>(v);  // by 1, 2, 4, 8 lanes inside each quad
+    v += shifted<0x112, 0xF>(v);
+    v += shifted<0x114, 0xF>(v);
+    v += shifted<0x118, 0xF>(v);
+    v += shifted<0x142, 0xA>(v);  // the last lane of quads 0 and 2 to quads 1 and 3
+    return v + shifted<0x143, 0xC>(v);  // lane 31 to quads 2 and 3
 }
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, rotated<8>(v));
@@ -79,12 +93,15 @@ __device__ __forceinline__ int window_begin(const AttentionKv4Args &a, int pos) 
 // (group, row) pairs as the 16 columns of the operand: one instruction multiplies a row tile's weights of all groups in the
 // set, of which each dim uses its own group's.
 //
-// The positions of all sequences are one line of steps, cut into equal pieces, one per workgroup (each kv head its own
-// line): however ragged the batch, all workgroups end together. A piece may end inside a sequence and begin inside another;
-// its stretch of a sequence is a segment. A sequence that lies in one piece is stored at once, the segments of others are
-// joined by a second launch. The four waves of a workgroup take the steps of a segment in turn and meet in LDS.
+// The positions of all sequences are one line of steps, cut into equal pieces, one per wave (each kv head its own line):
+// however ragged the batch, all waves end together. A piece may end inside a sequence and begin inside another; its stretch
+// of a sequence is a segment. A sequence that lies in one piece is stored at once, the segments of others are joined by a
+// second launch. A wave is a workgroup of its own: nothing waits for another wave. Short contexts (at most kAloneSteps steps)
+// take the other form: a workgroup of kAloneWaves waves has a whole row tile, the waves take its steps in turn and meet in
+// LDS, and there is no second launch (517 positions, 8 kv heads: 11 us and 8 + 4 us).
+constexpr int kAloneWaves = 8, kAloneSteps = 16;
 struct DecodePlan {
-    int workers;  // workgroups per kv head
+    int workers;  // waves per kv head
     int tiles;    // row tiles per sequence; row tile t of sequence b is number b * tiles + t of the line
     int least;    // steps that a piece has at least
     int alone;    // every workgroup has a whole row tile (no second launch)
@@ -99,9 +116,8 @@ struct Decode {
     static constexpr int kSets = kColumns / 16, kSetGroups = kGroups / kSets;
     static constexpr int kSetWords = 4 * kSetGroups, kLanesPerWord = 16 / kSetWords, kNibbles = 8 / kLanesPerWord;
     static constexpr int kRowBytes = 4 * kColumns + 16;  // of a position's weights in LDS: both pieces, 16 bytes off a power of two
-    static constexpr int kWaveBytes = kStep * kRowBytes;
-    static constexpr int kJoinBytes = kWaves * kRows * kDim * 4;
-    static constexpr int kLds = kWaves * kWaveBytes > kJoinBytes ? kWaves * kWaveBytes : kJoinBytes;
+    static constexpr int kLds = kStep * kRowBytes;
+    static_assert(kLds >= 4 * (kGroups * 4 + 8) * 4, "the sums of four quads");
     using KeyWords = typename std::conditional<kGroups == 4, uint4_t, uint2_t>::type;
     struct Places {
         uint32_t block[kTiles], slot[kTiles];  // of each tile of 16 positions: page * n_kv_heads + head, first slot
@@ -133,6 +149,19 @@ struct RowTile {
         first_step = lo / step;
         steps = rows_left > 0 && hi > lo ? (hi + step - 1) / step - first_step : 0;
     }
+    RowTile() = default;
+    __device__ RowTile of_lane(int lane) const {
+        RowTile t;
+        t.row0 = __builtin_amdgcn_readlane(row0, lane);
+        t.rows_left = __builtin_amdgcn_readlane(rows_left, lane);
+        t.first_row = __builtin_amdgcn_readlane(first_row, lane);
+        t.pos0 = __builtin_amdgcn_readlane(pos0, lane);
+        t.pos_low = __builtin_amdgcn_readlane(pos_low, lane);
+        t.pos_high = __builtin_amdgcn_readlane(pos_high, lane);
+        t.first_step = __builtin_amdgcn_readlane(first_step, lane);
+        t.steps = __builtin_amdgcn_readlane(steps, lane);
+        return t;
+    }
 };
 
 // Where segments and what joins them lie in the workspace. A segment has the number worker + row tile (unique: from one
@@ -161,59 +190,66 @@ __device__ __forceinline__ void store_row(const AttentionKv4Args &a, size_t quer
     *(uint2_t *)(a.output + query * a.output_stride + (size_t)head * a.cache.head_dim + d) = packed;
 }
 
-template <int kDim, int kRows>
-__global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const AttentionKv4Args a, const DecodePlan plan) {
+template <int kDim, int kRows, int kWaves>
+__global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(const AttentionKv4Args a, const DecodePlan plan) {
     using D = Decode<kDim, kRows>;
     constexpr int G = D::kGroups;
-    __shared__ __align__(16) unsigned char lds[D::kLds];
-    __shared__ float join_base[kWaves][kRows], join_sum[kWaves][kRows];
+    constexpr bool kAlone = kWaves > 1;
+    constexpr int kJoin = kAlone ? kWaves * kRows * kDim * 4 : 0;
+    __shared__ __align__(16) unsigned char lds_all[kWaves * D::kLds > kJoin ? kWaves * D::kLds : kJoin];
+    __shared__ float2 join_bases[kAlone ? kWaves : 1][kRows];
     const Kv4Cache &c = a.cache;
-    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int quad = lane >> 4, t16 = lane & 15;
+    const int lane = threadIdx.x % kWave, quad = lane >> 4, t16 = lane & 15;
+    const int wave = kAlone ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : 0;
+    unsigned char *lds = lds_all + wave * D::kLds;
     const int kv = blockIdx.x, worker = blockIdx.y + blockIdx.z * gridDim.y;  // kv fastest: a head's pieces fall on the same XCDs
     if (worker >= plan.workers) return;
     const int heads = a.n_heads / c.n_kv_heads, numbers = a.batch.batch * plan.tiles;
 
-    // this workgroup's piece of the line, and the row tile that it begins in
+    // this wave's piece of the line, and the row tile that it begins in
     int number = worker, offset = 0, left = INT32_MAX;
-    if (!plan.alone) {
+    RowTile tile;
+    if constexpr (kAlone) {
+        tile = RowTile(a, plan, number, kRows, D::kStep);
+        if (tile.rows_left <= 0) return;
+    } else {
         int total = 0;
-        for (int base = 0; base < numbers; base += kWave)
-            total += base + lane < numbers ? RowTile(a, plan, base + lane, kRows, D::kStep).steps : 0;
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) total += __shfl_xor(total, off, kWave);
+        RowTile own;
+        const auto running = [&](int base) {
+            own.steps = 0;
+            if (base + lane < numbers) own = RowTile(a, plan, base + lane, kRows, D::kStep);
+            return running_sum(own.steps);
+        };
+        int upto = 0;
+        for (int base = 0; base < numbers; base += kWave) {
+            upto = running(base);
+            total += __builtin_amdgcn_readlane(upto, kWave - 1);
+        }
         const int per = max(plan.least, (total + plan.workers - 1) / plan.workers);
         const long long begin = (long long)worker * per;
-        const bool scribe = kv == 0 && worker == 0 && wave == 0;
+        const bool scribe = kv == 0 && worker == 0;
         left = (int)min((long long)per, total - begin);
-        if (left <= 0 && !(kv == 0 && worker == 0)) return;
+        if (left <= 0 && !scribe) return;
         const Segments segments(a, plan, kRows);
-        int before = 0;
-        number = -1;
-        for (int base = 0; base < numbers && (number < 0 || scribe); base += kWave) {
-            const int steps = base + lane < numbers ? RowTile(a, plan, base + lane, kRows, D::kStep).steps : 0;
-            int upto = steps;
-#pragma unroll
-            for (int off = 1; off < kWave; off <<= 1) {
-                const int v = __shfl_up(upto, off, kWave);
-                upto += lane >= off ? v : 0;
-            }
-            const int from = before + upto - steps;
+        int before = 0, at = -1;
+        for (int base = 0; base < numbers && (at < 0 || scribe); base += kWave) {
+            if (numbers > kWave) upto = running(base);
+            const int from = before + upto - own.steps;
             if (scribe && base + lane < numbers)
-                segments.parts[base + lane] = make_int2(from / per, steps ? (from + steps - 1) / per - from / per + 1 : 0);
-            const unsigned long long here = __ballot(number < 0 && steps > 0 && begin >= from && begin < from + steps);
+                segments.parts[base + lane] = make_int2(from / per, own.steps ? (from + own.steps - 1) / per - from / per + 1 : 0);
+            const unsigned long long here = __ballot(at < 0 && own.steps > 0 && begin >= from && begin < from + own.steps);
             if (here) {
-                const int l = __ffsll((unsigned long long)here) - 1;
-                number = base + l;
-                offset = (int)begin - __shfl(from, l, kWave);
+                const int l = __builtin_amdgcn_readfirstlane(__ffsll(here) - 1);
+                at = base + l;
+                offset = (int)begin - __builtin_amdgcn_readlane(from, l);
+                tile = own.of_lane(l);
             }
-            before += __shfl(upto, kWave - 1, kWave);
+            before += __builtin_amdgcn_readlane(upto, kWave - 1);
         }
         if (left <= 0) return;  // (nothing at all to see)
+        number = __builtin_amdgcn_readfirstlane(at);
+        left = __builtin_amdgcn_readfirstlane(left);
     }
-    number = __builtin_amdgcn_readfirstlane(number);
-    offset = __builtin_amdgcn_readfirstlane(offset);
-    left = __builtin_amdgcn_readfirstlane(left);
 
     const int limit = position_limit(a);
     const int row_quad = quad % (kRows / 4), pack = quad / (kRows / 4);  // this lane's results: rows 4 * row_quad + r of tile `pack`
@@ -226,22 +262,19 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
     float minus_one = -1.0f;  // (a variable: the product with it is folded into a mixed-precision instruction, a difference is not)
     asm("" : "+v"(minus_one));
     const float c_low = a.scale * 1.44269504088896f, c_even = c_low * 16777216.0f, c_odd = c_low * 1048576.0f;
-    unsigned char *mine = lds + wave * D::kWaveBytes;
 
     while (true) {
-        const RowTile tile(a, plan, number, kRows, D::kStep);
         const int count = min(tile.steps - offset, left);
-        const bool entire = plan.alone || (offset == 0 && count == tile.steps);
-        if (tile.rows_left <= 0) return;  // (alone only)
+        const bool entire = kAlone || (offset == 0 && count == tile.steps);
         const int *table = a.batch.table + (size_t)(plan.tiles == 1 ? number : number / plan.tiles) * a.batch.width;
 
         // 64 entries of the page table at a time, one per lane: a step's pages are then a lane read away (a load of their own
         // would stand in front of every step's loads)
-        int held_from = INT32_MIN, held = -1;
+        int held_from = (tile.first_step + offset) * D::kStep >> c.page_shift, held = table[min(held_from + lane, a.batch.width - 1)];
         auto find = [&](int step) {
             typename D::Places x;
             const int at = step * D::kStep, last = (at + 16 * (D::kTiles - 1)) >> c.page_shift;
-            if (held_from == INT32_MIN || last >= held_from + kWave) {
+            if (last >= held_from + kWave) {
                 held_from = at >> c.page_shift;
                 held = table[min(held_from + lane, a.batch.width - 1)];
             }
@@ -298,13 +331,6 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
 
         int step = tile.first_step + offset + wave;
         const int end = tile.first_step + offset + count;
-        typename D::Places at;
-        typename D::Keys now;
-        if (step < end) {
-            at = find(step);
-            load_keys(now, at);
-        }
-
         // row operands: this lane's row and its 8 dims of each group; and the groups' sums, which the minima multiply, as one
         // more operand: first and second fp16 piece of sum / 32 at the depth of the quad that holds the minima of the row's tile
         // (rows that are not there are zeros; what they see shows in their own columns only)
@@ -316,6 +342,17 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
 #pragma unroll
             for (int g = 0; g < G; g++) {
                 q[g] = real ? *(const half8_t *)(src + g * 32) : half8_t{};
+            }
+        }
+        typename D::Places at;
+        typename D::Keys now;
+        if (step < end) {
+            at = find(step);
+            load_keys(now, at);
+        }
+        {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
                 float sum = 0;
 #pragma unroll
                 for (int j = 0; j < 8; j++) sum += (float)q[g][j];
@@ -474,7 +511,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
                     w[r] = __builtin_amdgcn_exp2f(raw[p][r] - base[r]);
                     sum[r] += w[r];
                 }
-                unsigned char *to = mine + (16 * (p * D::kPack + pack) + t16) * D::kRowBytes + row_quad * 8;
+                unsigned char *to = lds + (16 * (p * D::kPack + pack) + t16) * D::kRowBytes + row_quad * 8;
 #pragma unroll
                 for (int g = 0; g < G; g++) {
                     const float size = low_half(now.vm[p][g]) * sign, low = __builtin_fmaf(low_half(now.vm[p][g]), flipped, high_half(now.vm[p][g]));
@@ -509,7 +546,7 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
                         short4_t two[2];
 #pragma unroll
                         for (int i = 0; i < 2; i++) {
-                            unsigned char *from = mine + (16 * (2 * half + i) + 4 * quad + (lane >> 2 & 3)) * D::kRowBytes + piece * D::kColumns * 2 + e * 32 + (lane & 3) * 8;
+                            unsigned char *from = lds + (16 * (2 * half + i) + 4 * quad + (lane >> 2 & 3)) * D::kRowBytes + piece * D::kColumns * 2 + e * 32 + (lane & 3) * 8;
                             two[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)from);
                         }
                         struct Both { short4_t x[2]; } both = {{two[0], two[1]}};
@@ -542,123 +579,168 @@ __global__ __launch_bounds__(kThreads, 2) void attention_decode_kernel(const Att
             now = next;
         }
 
-        // ---- the wave's sums over its lanes
+        // ---- the sums of weights and minima over the lanes: inside each quad, then through LDS. A lane's results are column
+        // (group in the set, row); of its set's groups a dim has one, and all dims of the quad the same: other lanes have none.
+        const int row = t16 % kRows, in_set = t16 / kRows;
+        constexpr int kQuadFloats = G * 4 + 8;  // minima [group][row], sums, bases
+        float *quads = (float *)lds;
 #pragma unroll
         for (int r = 0; r < 4; r++) {
             sum[r] = quad_sum(sum[r]);
 #pragma unroll
             for (int g = 0; g < G; g++) acc_min[g][r] = quad_sum(acc_min[g][r]);
-#pragma unroll
-            for (int off = 4 * kRows; off < kWave; off <<= 1) {
-                sum[r] += __shfl_xor(sum[r], off, kWave);
-#pragma unroll
-                for (int g = 0; g < G; g++) acc_min[g][r] += __shfl_xor(acc_min[g][r], off, kWave);
-            }
         }
-        if (t16 == 0 && pack == 0) {
+        if (t16 == 0) {
+            float4_t *to = (float4_t *)(quads + quad * kQuadFloats);
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                join_base[wave][4 * row_quad + r] = base[r];
-                join_sum[wave][4 * row_quad + r] = sum[r];
-            }
+            for (int g = 0; g < G; g++) to[g] = float4_t{acc_min[g][0], acc_min[g][1], acc_min[g][2], acc_min[g][3]};
+            to[G] = float4_t{sum[0], sum[1], sum[2], sum[3]};
+            to[G + 1] = float4_t{base[0], base[1], base[2], base[3]};
         }
-        // this lane's column is (group in the set, row): the minima's share of each set's group
-        const int row = t16 % kRows, in_set = t16 / kRows;
-        float low[D::kSets];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        float total = 0, low[D::kSets] = {};
+        const float *from = quads + (row >> 2) * kQuadFloats + (row & 3);
 #pragma unroll
-        for (int e = 0; e < D::kSets; e++) {
-            low[e] = 0;
+        for (int u = 0; u < D::kPack; u++) {
+            const float *one = from + u * (kRows / 4) * kQuadFloats;
+            total += one[G * 4];
 #pragma unroll
-            for (int g = 0; g < D::kSetGroups; g++)
+            for (int e = 0; e < D::kSets; e++) low[e] += one[(e * D::kSetGroups + (in_set < D::kSetGroups ? in_set : 0)) * 4];
+        }
+        const float own_base = from[G * 4 + 4];
+        if constexpr (kAlone) __syncthreads();  // every wave is through with its weights and sums
+        if (row < tile.rows_left && in_set == quad * D::kSetGroups / 4) {
+            const Segments segments(a, plan, kRows);
+            const int at_row = tile.first_row + row;
+            const size_t query = (size_t)(tile.row0 + at_row / heads);
+            const int head = kv * heads + at_row % heads;
+            const size_t slot = ((size_t)kv * segments.per_head + worker + number) * kRows + row;
+            if (!entire && quad * D::kSetGroups % 4 == 0 && in_set == 0) *(float2 *)(segments.bases + slot * 2) = make_float2(own_base, total);
+            if (kAlone && quad * D::kSetGroups % 4 == 0 && in_set == 0) join_bases[wave][row] = make_float2(own_base, total);
+#pragma unroll
+            for (int e = 0; e < D::kSets; e++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const float v = __shfl(acc_min[e * D::kSetGroups + g][r], (row >> 2) * 16, kWave);
-                    if (in_set == g && (row & 3) == r) low[e] = v;
+                    const int n = 4 * quad + r;  // the operand's row: word n / kLanesPerWord of the set, part n % kLanesPerWord of it
+                    const int d = (e * D::kSetWords + n / D::kLanesPerWord) * 8 + n % D::kLanesPerWord * D::kNibbles;
+                    float v[D::kNibbles];
+#pragma unroll
+                    for (int i = 0; i < D::kNibbles; i++) v[i] = __builtin_fmaf(acc[e][i][r], 1048576.0f, low[e]);
+                    if constexpr (kAlone) {
+                        float *to = (float *)lds_all + ((size_t)wave * kRows + row) * kDim + d;
+#pragma unroll
+                        for (int i = 0; i < D::kNibbles; i++) to[i] = v[i];
+                    } else if (entire) {
+                        uint16_t *to = a.output + query * a.output_stride + (size_t)head * kDim + d;
+                        const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // nothing seen: 0
+#pragma unroll
+                        for (int i = 0; i < D::kNibbles; i += 2) ((uint32_t *)to)[i / 2] = (uint32_t)f2h(v[i] * inv) | (uint32_t)f2h(v[i + 1] * inv) << 16;
+                    } else {
+                        float *to = segments.sums + slot * kDim + d;
+#pragma unroll
+                        for (int i = 0; i < D::kNibbles; i++) to[i] = v[i];
+                    }
                 }
         }
-        __syncthreads();  // (also: every wave is through with its weights in LDS)
-        float highest = kEmpty;
+        if constexpr (kAlone) {
+            __syncthreads();
+            constexpr int kParts = kDim / 4;  // float4s of a row
+            for (int j = threadIdx.x; j < kRows * kParts; j += kWaves * kWave) {
+                const int r = j / kParts, d = j % kParts * 4;
+                if (r >= tile.rows_left) break;
+                float m = kEmpty, all = 0;
+                float4_t o = {};
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) highest = fmaxf(highest, join_base[w][row]);
-        const float mine_keep = __builtin_amdgcn_exp2f(join_base[wave][row] - highest);
-        float *out = (float *)lds + (size_t)wave * kRows * kDim + row * kDim;
+                for (int w = 0; w < kWaves; w++) m = fmaxf(m, join_bases[w][r].x);
 #pragma unroll
-        for (int e = 0; e < D::kSets; e++)
-#pragma unroll
-            for (int i = 0; i < D::kNibbles; i++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int n = 4 * quad + r;  // the operand's row: word n / kLanesPerWord of the set, nibble part n % kLanesPerWord
-                    const int dim = (e * D::kSetWords + n / D::kLanesPerWord) * 8 + n % D::kLanesPerWord * D::kNibbles + i;
-                    if (in_set < D::kSetGroups && dim / 32 - e * D::kSetGroups == in_set) out[dim] = __builtin_fmaf(acc[e][i][r], 1048576.0f, low[e]) * mine_keep;
+                for (int w = 0; w < kWaves; w++) {
+                    const float keep = __builtin_amdgcn_exp2f(join_bases[w][r].x - m);
+                    all += join_bases[w][r].y * keep;
+                    o += *(const float4_t *)((const float *)lds_all + ((size_t)w * kRows + r) * kDim + d) * keep;
                 }
-        __syncthreads();
-        constexpr int kParts = kDim / 4;  // float4s of a row
-        for (int j = threadIdx.x; j < kRows * kParts; j += kThreads) {
-            const int r = j / kParts, d = j % kParts * 4;
-            if (r >= tile.rows_left) break;
-            float4_t o = {};
-            float m = kEmpty, total = 0;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                o += *(const float4_t *)((const float *)lds + (size_t)w * kRows * kDim + r * kDim + d);
-                m = fmaxf(m, join_base[w][r]);
-            }
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) total += join_sum[w][r] * __builtin_amdgcn_exp2f(join_base[w][r] - m);
-            if (entire) {
                 const int at_row = tile.first_row + r;
-                store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d, o, total);
-            } else {
-                const Segments segments(a, plan, kRows);
-                const size_t slot = ((size_t)kv * segments.per_head + worker + number) * kRows + r;
-                if (d == 0) *(float2 *)(segments.bases + slot * 2) = make_float2(m, total);
-                *(float4_t *)(segments.sums + slot * kDim + d) = o;
+                store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d, o, all);
             }
+            return;
         }
         left -= count;
-        if (plan.alone || left <= 0) return;
+        if (left <= 0) return;
         offset = 0;
         do {
             if (++number >= numbers) return;
-        } while (RowTile(a, plan, number, kRows, D::kStep).steps == 0);
-        __syncthreads();
+            tile = RowTile(a, plan, number, kRows, D::kStep);
+        } while (tile.steps == 0);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
-// Joins the segments of four rows of a row tile; writes the zeros of rows that see nothing. kDim / 4 lanes a row, the
-// segments dealt to kAtOnce groups of lanes, so that a long row's are read in few round trips.
-constexpr int kJoinThreads = 512;
-template <int kDim, int kRows>
+// Joins the segments of four rows of a row tile, or writes the zeros of rows that see nothing. kLanes lanes a row and
+// segment: kDim / 4 for all dims, or 8 and a workgroup for every 32 dims, which makes enough of them even for one sequence,
+// whose hundreds of segments are then read in a few round trips.
+constexpr int kJoinThreads = 256;
+template <int kDim, int kRows, int kLanes>
 __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttentionKv4Args a, const DecodePlan plan) {
-    constexpr int kLanes = kDim / 4, kAtOnce = kJoinThreads / (4 * kLanes);
+    constexpr int kAtOnce = kJoinThreads / (4 * kLanes), kParts = kDim / (4 * kLanes), kJoinWaves = kJoinThreads / kWave;
+    extern __shared__ float weights[];  // [4][parts]
+    __shared__ float highest[4][kJoinWaves], totals[4][kJoinWaves];
     __shared__ float4_t sums[kAtOnce][4][kLanes];
-    const int number = blockIdx.x, kv = blockIdx.y;
+    const int number = blockIdx.x, kv = blockIdx.y, first_row = blockIdx.z / kParts * 4, first_dim = blockIdx.z % kParts * 4 * kLanes;
     const Segments segments(a, plan, kRows);
     const int2 parts = segments.parts[number];
-    if (parts.y == 1) return;  // stored at once
     const RowTile tile(a, plan, number, kRows, Decode<kDim, kRows>::kStep);
-    const int d = threadIdx.x % kLanes, r = blockIdx.z * 4 + threadIdx.x / kLanes % 4, group = threadIdx.x / (4 * kLanes);
-    const int heads = a.n_heads / a.cache.n_kv_heads;
-    if ((int)blockIdx.z * 4 >= tile.rows_left) return;
-    float m = kEmpty, total = 0;
-    const size_t slot = ((size_t)kv * segments.per_head + parts.x + number) * kRows + r;
+    if (parts.y == 1 || first_row >= tile.rows_left) return;  // stored at once; no such rows
+    const size_t slot = ((size_t)kv * segments.per_head + parts.x + number) * kRows + first_row;
     const float2 *bases = (const float2 *)segments.bases + slot;
-#pragma unroll 8
-    for (int p = 0; p < parts.y; p++) m = fmaxf(m, bases[(size_t)p * kRows].x);
-#pragma unroll 8
-    for (int p = 0; p < parts.y; p++) total += bases[(size_t)p * kRows].y * __builtin_amdgcn_exp2f(bases[(size_t)p * kRows].x - m);
-    const float4_t *from = (const float4_t *)(segments.sums + slot * kDim) + d;
+    float m[4] = {kEmpty, kEmpty, kEmpty, kEmpty}, total[4] = {};
+    const int wave = threadIdx.x / kWave;
+    for (int p = threadIdx.x; p < parts.y; p += kJoinThreads)
+#pragma unroll
+        for (int r = 0; r < 4; r++) m[r] = fmaxf(m[r], bases[(size_t)p * kRows + r].x);
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        m[r] = quad_max(m[r]);
+        m[r] = fmaxf(m[r], __shfl_xor(m[r], 16, kWave));
+        m[r] = fmaxf(m[r], __shfl_xor(m[r], 32, kWave));
+        if (threadIdx.x % kWave == 0) highest[r][wave] = m[r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int w = 0; w < kJoinWaves; w++) m[r] = fmaxf(m[r], highest[r][w]);
+    for (int p = threadIdx.x; p < parts.y; p += kJoinThreads)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float2 one = bases[(size_t)p * kRows + r];
+            const float w = __builtin_amdgcn_exp2f(one.x - m[r]);
+            weights[r * parts.y + p] = w;
+            total[r] += one.y * w;
+        }
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        total[r] = quad_sum(total[r]);
+        total[r] += __shfl_xor(total[r], 16, kWave);
+        total[r] += __shfl_xor(total[r], 32, kWave);
+        if (threadIdx.x % kWave == 0) totals[r][wave] = total[r];
+    }
+    __syncthreads();
+    const int d = threadIdx.x % kLanes, r = threadIdx.x / kLanes % 4, group = threadIdx.x / (4 * kLanes);
+    const float4_t *from = (const float4_t *)(segments.sums + (slot + r) * kDim + first_dim) + d;
     float4_t o = {};
 #pragma unroll 8
-    for (int p = group; p < parts.y; p += kAtOnce) o += from[(size_t)p * kRows * kLanes] * __builtin_amdgcn_exp2f(bases[(size_t)p * kRows].x - m);
-    sums[group][r & 3][d] = o;
+    for (int p = group; p < parts.y; p += kAtOnce) o += from[(size_t)p * kRows * (kDim / 4)] * weights[r * parts.y + p];
+    sums[group][r][d] = o;
     __syncthreads();
-    if (group || r >= tile.rows_left) return;
+    if (group || first_row + r >= tile.rows_left) return;
 #pragma unroll
-    for (int j = 1; j < kAtOnce; j++) o += sums[j][r & 3][d];
-    const int at_row = tile.first_row + r;
-    store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d * 4, o, total);
+    for (int j = 1; j < kAtOnce; j++) o += sums[j][r][d];
+    float all = 0;
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; w++) all += totals[r][w];
+    const int heads = a.n_heads / a.cache.n_kv_heads, at_row = tile.first_row + first_row + r;
+    store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, first_dim + d * 4, o, all);
 }
 
 int decode_rows(const AttentionKv4Args &a) {
@@ -671,12 +753,12 @@ DecodePlan decode_plan(const AttentionKv4Args &a) {
     const long long heads = a.n_heads / a.cache.n_kv_heads;
     DecodePlan p;
     p.tiles = (int)((a.max_query * heads + rows - 1) / rows);
-    p.least = 2 * kWaves;
+    p.least = 1;
     long long reach = a.max_length;  // positions that a row tile may see, and the steps that they may touch
     if (a.window > 0 && (long long)a.window + a.max_query < reach) reach = (long long)a.window + a.max_query;
     const long long steps = (reach + step - 1) / step + 1;
-    p.alone = steps <= 4 * kWaves;
-    const int slots = 2 * current_device_cus();
+    p.alone = steps <= kAloneSteps;
+    const int slots = 8 * std::min(current_device_cus(), 256);  // two waves a SIMD; the join holds a weight per worker in LDS
     p.workers = p.alone ? a.batch.batch * p.tiles : (slots + a.cache.n_kv_heads - 1) / a.cache.n_kv_heads;
     return p;
 }
@@ -684,12 +766,19 @@ DecodePlan decode_plan(const AttentionKv4Args &a) {
 template <int kDim, int kRows>
 hipError_t launch_decode_rows(const AttentionKv4Args &a, const DecodePlan &plan, hipStream_t s) {
     const int across = plan.workers < 32768 ? plan.workers : 32768;
-    attention_decode_kernel<kDim, kRows><<<dim3((unsigned)a.cache.n_kv_heads, (unsigned)across, (unsigned)((plan.workers + across - 1) / across)), kThreads, 0, s>>>(a, plan);
-    if (!plan.alone) {
-        const dim3 grid((unsigned)(a.batch.batch * plan.tiles), (unsigned)a.cache.n_kv_heads, kRows / 4);
-        if (hipError_t e = hipGetLastError()) return e;
-        attention_join_kernel<kDim, kRows><<<grid, kJoinThreads, 0, s>>>(a, plan);
+    const dim3 grid((unsigned)a.cache.n_kv_heads, (unsigned)across, (unsigned)((plan.workers + across - 1) / across));
+    if (plan.alone) {
+        attention_decode_kernel<kDim, kRows, kAloneWaves><<<grid, kAloneWaves * kWave, 0, s>>>(a, plan);
+        return hipGetLastError();
     }
+    attention_decode_kernel<kDim, kRows, 1><<<grid, kWave, 0, s>>>(a, plan);
+    if (hipError_t e = hipGetLastError()) return e;
+    const unsigned tiles = (unsigned)(a.batch.batch * plan.tiles), kv = (unsigned)a.cache.n_kv_heads;
+    const size_t lds = 16 * (size_t)plan.workers;
+    if ((long long)tiles * kv * (kRows / 4) < current_device_cus())
+        attention_join_kernel<kDim, kRows, 8><<<dim3(tiles, kv, kRows / 4 * (kDim / 32)), kJoinThreads, lds, s>>>(a, plan);
+    else
+        attention_join_kernel<kDim, kRows, kDim / 4><<<dim3(tiles, kv, kRows / 4), kJoinThreads, lds, s>>>(a, plan);
     return hipGetLastError();
 }
 
