@@ -100,11 +100,12 @@ __device__ __forceinline__ int window_begin(const AttentionKv4Args &a, int pos) 
 // take the other form: a workgroup of kAloneWaves waves has a whole row tile, the waves take its steps in turn and meet in
 // LDS, and there is no second launch (517 positions, 8 kv heads: 11 us and 8 + 4 us).
 constexpr int kAloneWaves = 8, kAloneSteps = 16;
-struct DecodePlan {
+struct RowPlan {
     int workers;  // waves per kv head
     int tiles;    // row tiles per sequence; row tile t of sequence b is number b * tiles + t of the line
     int least;    // steps that a piece has at least
     int alone;    // every workgroup has a whole row tile (no second launch)
+    int from_rows, to_rows;  // sequences with from_rows <= rows < to_rows are this launch's, rows counted with the heads
 };
 
 template <int kDim, int kRows>
@@ -135,14 +136,14 @@ struct Decode {
 // One row tile: its rows and the steps of positions that some row of it sees.
 struct RowTile {
     int row0, rows_left, first_row, pos0, pos_low, pos_high, first_step, steps;
-    __device__ RowTile(const AttentionKv4Args &a, const DecodePlan &plan, int number, int rows_per_tile, int step) {
+    __device__ RowTile(const AttentionKv4Args &a, const RowPlan &plan, int number, int rows_per_tile, int step) {
         const int seq = plan.tiles == 1 ? number : number / plan.tiles, tile = plan.tiles == 1 ? 0 : number - seq * plan.tiles;
         const int heads = a.n_heads / a.cache.n_kv_heads;
         const Sequence s(a, seq);
         row0 = s.row0;
         pos0 = s.pos0;
         first_row = tile * rows_per_tile;
-        rows_left = s.rows * heads - first_row;
+        rows_left = s.rows * heads >= plan.from_rows && s.rows * heads < plan.to_rows ? s.rows * heads - first_row : 0;
         pos_low = s.pos0 + first_row / heads;
         pos_high = s.pos0 + (first_row + min(rows_left, rows_per_tile) - 1) / heads;
         const int lo = window_begin(a, pos_low), hi = min(pos_high + 1, position_limit(a));
@@ -170,19 +171,59 @@ struct Segments {
     float *sums, *bases;
     int2 *parts;  // of each row tile: first worker, and how many (0: it sees nothing)
     int per_head;
-    __host__ __device__ Segments(const AttentionKv4Args &a, const DecodePlan &plan, int rows) {
+    __host__ __device__ Segments(const AttentionKv4Args &a, const RowPlan &plan, int rows, size_t at = 0) {
         const int numbers = a.batch.batch * plan.tiles;
         per_head = plan.workers + numbers;
         const size_t all = (size_t)a.cache.n_kv_heads * per_head * rows;
-        sums = (float *)a.workspace;
+        sums = (float *)((char *)a.workspace + at);
         bases = sums + all * a.cache.head_dim;
         parts = (int2 *)(bases + all * 2);
     }
-    __host__ __device__ static size_t bytes(const AttentionKv4Args &a, const DecodePlan &plan, int rows) {
+    __host__ __device__ static size_t bytes(const AttentionKv4Args &a, const RowPlan &plan, int rows) {
         const size_t numbers = (size_t)a.batch.batch * plan.tiles;
         return (size_t)a.cache.n_kv_heads * (plan.workers + numbers) * rows * (a.cache.head_dim + 2) * 4 + numbers * 8;
     }
 };
+
+// The worker's piece of the line: `left` steps from step `offset` of row tile `number` on; false if it has none. With
+// `parts`, the wave also writes down for every row tile which workers have parts of it. All lanes take part.
+__device__ __forceinline__ bool find_piece(const AttentionKv4Args &a, const RowPlan &plan, int worker, int rows, int step, bool first,
+                                           int2 *parts, int *number, int *offset, int *left, RowTile *tile) {
+    const int lane = threadIdx.x % kWave, numbers = a.batch.batch * plan.tiles;
+    RowTile own;
+    const auto running = [&](int base) {
+        own.steps = 0;
+        if (base + lane < numbers) own = RowTile(a, plan, base + lane, rows, step);
+        return running_sum(own.steps);
+    };
+    int total = 0, upto = 0;
+    for (int base = 0; base < numbers; base += kWave) {
+        upto = running(base);
+        total += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    const int per = max(plan.least, (total + plan.workers - 1) / plan.workers);
+    const long long begin = (long long)worker * per;
+    const int n = (int)min((long long)per, total - begin);
+    if (n <= 0 && !first) return false;
+    int before = 0, at = -1;
+    for (int base = 0; base < numbers && (at < 0 || parts); base += kWave) {
+        if (numbers > kWave) upto = running(base);
+        const int from = before + upto - own.steps;
+        if (parts && base + lane < numbers)
+            parts[base + lane] = make_int2(from / per, own.steps ? (from + own.steps - 1) / per - from / per + 1 : 0);
+        const unsigned long long here = __ballot(at < 0 && own.steps > 0 && begin >= from && begin < from + own.steps);
+        if (here) {
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll(here) - 1);
+            at = base + l;
+            *offset = (int)begin - __builtin_amdgcn_readlane(from, l);
+            *tile = own.of_lane(l);
+        }
+        before += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    *number = __builtin_amdgcn_readfirstlane(at);
+    *left = __builtin_amdgcn_readfirstlane(n);
+    return n > 0;  // (none at all to see: only the parts were written)
+}
 
 __device__ __forceinline__ void store_row(const AttentionKv4Args &a, size_t query, int head, int d, float4_t o, float total) {
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // nothing seen: 0
@@ -191,7 +232,7 @@ __device__ __forceinline__ void store_row(const AttentionKv4Args &a, size_t quer
 }
 
 template <int kDim, int kRows, int kWaves>
-__global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(const AttentionKv4Args a, const DecodePlan plan) {
+__global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(const AttentionKv4Args a, const RowPlan plan) {
     using D = Decode<kDim, kRows>;
     constexpr int G = D::kGroups;
     constexpr bool kAlone = kWaves > 1;
@@ -213,42 +254,9 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
         tile = RowTile(a, plan, number, kRows, D::kStep);
         if (tile.rows_left <= 0) return;
     } else {
-        int total = 0;
-        RowTile own;
-        const auto running = [&](int base) {
-            own.steps = 0;
-            if (base + lane < numbers) own = RowTile(a, plan, base + lane, kRows, D::kStep);
-            return running_sum(own.steps);
-        };
-        int upto = 0;
-        for (int base = 0; base < numbers; base += kWave) {
-            upto = running(base);
-            total += __builtin_amdgcn_readlane(upto, kWave - 1);
-        }
-        const int per = max(plan.least, (total + plan.workers - 1) / plan.workers);
-        const long long begin = (long long)worker * per;
         const bool scribe = kv == 0 && worker == 0;
-        left = (int)min((long long)per, total - begin);
-        if (left <= 0 && !scribe) return;
         const Segments segments(a, plan, kRows);
-        int before = 0, at = -1;
-        for (int base = 0; base < numbers && (at < 0 || scribe); base += kWave) {
-            if (numbers > kWave) upto = running(base);
-            const int from = before + upto - own.steps;
-            if (scribe && base + lane < numbers)
-                segments.parts[base + lane] = make_int2(from / per, own.steps ? (from + own.steps - 1) / per - from / per + 1 : 0);
-            const unsigned long long here = __ballot(at < 0 && own.steps > 0 && begin >= from && begin < from + own.steps);
-            if (here) {
-                const int l = __builtin_amdgcn_readfirstlane(__ffsll(here) - 1);
-                at = base + l;
-                offset = (int)begin - __builtin_amdgcn_readlane(from, l);
-                tile = own.of_lane(l);
-            }
-            before += __builtin_amdgcn_readlane(upto, kWave - 1);
-        }
-        if (left <= 0) return;  // (nothing at all to see)
-        number = __builtin_amdgcn_readfirstlane(at);
-        left = __builtin_amdgcn_readfirstlane(left);
+        if (!find_piece(a, plan, worker, kRows, D::kStep, scribe, scribe ? segments.parts : nullptr, &number, &offset, &left, &tile)) return;
     }
 
     const int limit = position_limit(a);
@@ -680,16 +688,16 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
 // segment: kDim / 4 for all dims, or 8 and a workgroup for every 32 dims, which makes enough of them even for one sequence,
 // whose hundreds of segments are then read in a few round trips.
 constexpr int kJoinThreads = 256;
-template <int kDim, int kRows, int kLanes>
-__global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttentionKv4Args a, const DecodePlan plan) {
+template <int kDim, int kRows, int kStep, int kLanes>
+__global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const AttentionKv4Args a, const RowPlan plan, size_t segments_at) {
     constexpr int kAtOnce = kJoinThreads / (4 * kLanes), kParts = kDim / (4 * kLanes), kJoinWaves = kJoinThreads / kWave;
     extern __shared__ float weights[];  // [4][parts]
     __shared__ float highest[4][kJoinWaves], totals[4][kJoinWaves];
     __shared__ float4_t sums[kAtOnce][4][kLanes];
     const int number = blockIdx.x, kv = blockIdx.y, first_row = blockIdx.z / kParts * 4, first_dim = blockIdx.z % kParts * 4 * kLanes;
-    const Segments segments(a, plan, kRows);
+    const Segments segments(a, plan, kRows, segments_at);
     const int2 parts = segments.parts[number];
-    const RowTile tile(a, plan, number, kRows, Decode<kDim, kRows>::kStep);
+    const RowTile tile(a, plan, number, kRows, kStep);
     if (parts.y == 1 || first_row >= tile.rows_left) return;  // stored at once; no such rows
     const size_t slot = ((size_t)kv * segments.per_head + parts.x + number) * kRows + first_row;
     const float2 *bases = (const float2 *)segments.bases + slot;
@@ -743,64 +751,403 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Atte
     store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, first_dim + d * 4, o, all);
 }
 
-int decode_rows(const AttentionKv4Args &a) {
-    const long long rows = (long long)a.max_query * (a.n_heads / a.cache.n_kv_heads);
-    return rows <= 4 ? 4 : rows <= 8 ? 8 : 16;
-}
+// ------------------------------------------------------------------------------------------------- many rows: prompts
+//
+// Bound: the matrix cores, 4 * kDim flops per row, head and seen position, with the vector pipe close behind (a score costs
+// some eight instructions, and a position's 4 kDim bits become 4 kDim bytes). A workgroup has 128 rows (query rows times the
+// heads that share a kv head), 32 per wave; tiles of kTile positions are brought to fp16 once for all of them, into LDS,
+// while the tile before is worked on. k and v are rounded to fp16 there, and p for the second product: three roundings of
+// 2^-12 (root mean square) next to the result's own; exact codes and two pieces of p, as for few rows, would cost as much
+// again as all the rest. Half of k and v are stored: m + 15 s may be half a step of s above fp16's largest.
+// Transposed products (k q^T, v^T p^T) put a row's scores into one lane and its partner 32 lanes on, and p is then the next
+// product's operand as it lies, if v's positions are ordered like the result rows of the first product (8 b + 4 h + r).
+template <int kDim>
+struct Prompt {
+    static constexpr int kGroups = kDim / kKvGroup, kWords = kDim / 8;
+    static constexpr int kTile = 8192 / kDim;  // 32 values of k and of v per thread
+    static constexpr int kWaves = 4, kThreads = kWaves * kWave, kRows = kWaves * 32;
+    static constexpr int kKeyBytes = kDim * 2 + 16, kValueBytes = kTile * 2 + 16;  // rows in LDS, off the banks' period
+    static constexpr int kKeyTile = kTile * kKeyBytes, kStage = kKeyTile + kDim * kValueBytes;
+    static constexpr int kSub = kTile / 32, kDepths = kDim / 16;
+};
+typedef float float16_t __attribute__((ext_vector_type(16)));
 
-DecodePlan decode_plan(const AttentionKv4Args &a) {
-    const int rows = decode_rows(a), step = rows == 4 ? 64 : 32;
-    const long long heads = a.n_heads / a.cache.n_kv_heads;
-    DecodePlan p;
-    p.tiles = (int)((a.max_query * heads + rows - 1) / rows);
-    p.least = 1;
-    long long reach = a.max_length;  // positions that a row tile may see, and the steps that they may touch
-    if (a.window > 0 && (long long)a.window + a.max_query < reach) reach = (long long)a.window + a.max_query;
-    const long long steps = (reach + step - 1) / step + 1;
-    p.alone = steps <= kAloneSteps;
-    const int slots = 8 * std::min(current_device_cus(), 256);  // two waves a SIMD; the join holds a weight per worker in LDS
-    p.workers = p.alone ? a.batch.batch * p.tiles : (slots + a.cache.n_kv_heads - 1) / a.cache.n_kv_heads;
-    return p;
-}
-
-template <int kDim, int kRows>
-hipError_t launch_decode_rows(const AttentionKv4Args &a, const DecodePlan &plan, hipStream_t s) {
-    const int across = plan.workers < 32768 ? plan.workers : 32768;
-    const dim3 grid((unsigned)a.cache.n_kv_heads, (unsigned)across, (unsigned)((plan.workers + across - 1) / across));
+template <int kDim>
+__global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const AttentionKv4Args a, const RowPlan plan, size_t segments_at) {
+    using P = Prompt<kDim>;
+    constexpr int G = P::kGroups;
+    __shared__ __align__(16) unsigned char stage[2][P::kStage];
+    __shared__ uint32_t unsound[2][P::kTile + 1];  // groups of each position's value that are not finite; and whether any is
+    const Kv4Cache &c = a.cache;
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5, l32 = lane & 31;
+    const int kv = blockIdx.x, worker = blockIdx.y + blockIdx.z * gridDim.y;
+    if (worker >= plan.workers) return;
+    const int heads = a.n_heads / c.n_kv_heads, numbers = a.batch.batch * plan.tiles;
+    int number, offset = 0, left = INT32_MAX;
+    RowTile tile;
     if (plan.alone) {
-        attention_decode_kernel<kDim, kRows, kAloneWaves><<<grid, kAloneWaves * kWave, 0, s>>>(a, plan);
-        return hipGetLastError();
+        // last tiles first: they see the most
+        number = worker % a.batch.batch * plan.tiles + plan.tiles - 1 - worker / a.batch.batch;
+        tile = RowTile(a, plan, number, P::kRows, P::kTile);
+        if (tile.rows_left <= 0) return;
+    } else {
+        const bool scribe = kv == 0 && worker == 0 && wave == 0;
+        const Segments segments(a, plan, P::kRows, segments_at);
+        if (!find_piece(a, plan, worker, P::kRows, P::kTile, kv == 0 && worker == 0, scribe ? segments.parts : nullptr, &number, &offset, &left, &tile)) return;
     }
-    attention_decode_kernel<kDim, kRows, 1><<<grid, kWave, 0, s>>>(a, plan);
-    if (hipError_t e = hipGetLastError()) return e;
-    const unsigned tiles = (unsigned)(a.batch.batch * plan.tiles), kv = (unsigned)a.cache.n_kv_heads;
-    const size_t lds = 16 * (size_t)plan.workers;
-    if ((long long)tiles * kv * (kRows / 4) < current_device_cus())
-        attention_join_kernel<kDim, kRows, 8><<<dim3(tiles, kv, kRows / 4 * (kDim / 32)), kJoinThreads, lds, s>>>(a, plan);
-    else
-        attention_join_kernel<kDim, kRows, kDim / 4><<<dim3(tiles, kv, kRows / 4), kJoinThreads, lds, s>>>(a, plan);
-    return hipGetLastError();
+    const int limit = position_limit(a);
+    const size_t code_words = kv4_code_words(1 << c.page_shift, kDim), scale_words = kv4_scale_words(1 << c.page_shift, kDim);
+    const float to_log2 = fabsf(a.scale) * (2.0f * 1.44269504088896f);  // (the sign is the row operand's)
+
+    while (true) {
+        const int count = min(tile.steps - offset, left);
+        const bool entire = plan.alone || (offset == 0 && count == tile.steps);
+        const int *table = a.batch.table + (size_t)(plan.tiles == 1 ? number : number / plan.tiles) * a.batch.width;
+        const int first = tile.first_step + offset, end = first + count;
+
+        // this lane's row, and its operand
+        const int in_tile = wave * 32 + l32, at_row = tile.first_row + in_tile;
+        const bool real = in_tile < tile.rows_left;
+        const size_t query = (size_t)(tile.row0 + (real ? at_row / heads : 0));
+        const int head = kv * heads + (real ? at_row % heads : 0), pos = real ? tile.pos0 + at_row / heads : -1;
+        half8_t q[P::kDepths];
+#pragma unroll
+        for (int k = 0; k < P::kDepths; k++) {
+            q[k] = real ? *(const half8_t *)(a.q + query * a.q_stride + (size_t)head * kDim + k * 16 + half * 8) : half8_t{};
+            if (a.scale < 0) q[k] = -q[k];
+        }
+        const int wave_rows = min(32, tile.rows_left - wave * 32);  // (none: the wave only helps with the tiles)
+        const int wave_low = tile.pos0 + (tile.first_row + wave * 32) / heads, wave_high = tile.pos0 + (tile.first_row + wave * 32 + max(wave_rows, 1) - 1) / heads;
+
+        int held_from = first * P::kTile >> c.page_shift, held = table[min(held_from + lane, a.batch.width - 1)];
+        struct Raw {
+            uint4_t k, v, v_scales;
+            uint32_t k_scales[4];
+            uint32_t there;  // bit i: positions 16 i .. 16 i + 15 have a page
+        };
+        // thread: 32 values of a position's key (one depth quad of every group; kDim 64: two positions) and of four positions' values
+        const int k_quad = threadIdx.x & 3, k_pos = threadIdx.x >> 2;
+        const int v_block = threadIdx.x % (P::kTile / 4), v_word = threadIdx.x / (P::kTile / 4);
+        auto load = [&](int step) {
+            Raw x;
+            const int at = step * P::kTile, last = (at + P::kTile - 16) >> c.page_shift;
+            if (last >= held_from + kWave) {
+                held_from = at >> c.page_shift;
+                held = table[min(held_from + lane, a.batch.width - 1)];
+            }
+            x.there = 0;
+#pragma unroll
+            for (int i = 0; i < P::kTile / 16; i++) {
+                const int index = (at + 16 * i) >> c.page_shift, page = __builtin_amdgcn_readlane(held, index - held_from);
+                x.there |= (uint32_t)(index < a.batch.width && page >= 0 && page < c.n_pages) << i;
+            }
+            auto block_of = [&](int t) {
+                const int page = __shfl(held, ((at + t) >> c.page_shift) - held_from, kWave);
+                return (size_t)((x.there >> (t / 16) & 1 ? page : 0) * c.n_kv_heads + kv);
+            };
+            const int slots = (1 << c.page_shift) - 1;
+            if constexpr (G == 4) {
+                const size_t b = block_of(k_pos);
+                const int slot = (at + k_pos) & slots;
+                x.k = *(const uint4_t *)(c.k_codes + b * code_words + (size_t)slot * P::kWords + k_quad * G);
+#pragma unroll
+                for (int g = 0; g < 4; g++) x.k_scales[g] = c.k_scales[b * scale_words + ((size_t)g << c.page_shift) + slot];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const size_t b = block_of(k_pos + 64 * i);
+                    const int slot = (at + k_pos + 64 * i) & slots;
+                    const uint2_t two = *(const uint2_t *)(c.k_codes + b * code_words + (size_t)slot * P::kWords + k_quad * G);
+                    x.k[2 * i] = two[0];
+                    x.k[2 * i + 1] = two[1];
+#pragma unroll
+                    for (int g = 0; g < 2; g++) x.k_scales[2 * i + g] = c.k_scales[b * scale_words + ((size_t)g << c.page_shift) + slot];
+                }
+            }
+            const size_t b = block_of(v_block * 4);
+            const int slot = (at + v_block * 4) & slots;
+            x.v = *(const uint4_t *)(c.v_codes + b * code_words + (size_t)slot * P::kWords + v_word * 4);
+            x.v_scales = *(const uint4_t *)(c.v_scales + b * scale_words + ((size_t)(v_word / 4) << c.page_shift) + slot);
+            return x;
+        };
+        // codes 1024 + c (64 + c from bits 4-7) less the rest, times s / 2, plus m / 2
+        auto value2 = [](uint32_t field, bool odd, half2_t s, half2_t m) {
+            const half2_t code = __builtin_bit_cast(half2_t, odd ? (field & kOddCodes) | 0x54005400u : (field & kEvenCodes) | 0x64006400u) - (odd ? half2_t{64, 64} : half2_t{1024, 1024});
+            return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, s, m));
+        };
+        auto store = [&](const Raw &x, int step, int into) {
+            const int at = step * P::kTile;
+            unsigned char *keys = stage[into], *values = stage[into] + P::kKeyTile;
+#pragma unroll
+            for (int pair = 0; pair < 2; pair++) {
+                const uint32_t w0 = x.k[2 * pair], w1 = x.k[2 * pair + 1];
+                const int to = G == 4 ? k_pos : k_pos + 64 * pair, group = G == 4 ? 2 * pair : 0;
+#pragma unroll
+                for (int odd = 0; odd < 2; odd++) {
+                    const half2_t both = __builtin_bit_cast(half2_t, x.k_scales[2 * pair + odd]) * half2_t{0.5f, 0.5f};
+                    const half2_t s = {both[0], both[0]}, m = {both[1], both[1]};
+                    const uint4_t out = {value2(w0, odd, s, m), value2(w0 >> 8, odd, s, m), value2(w1, odd, s, m), value2(w1 >> 8, odd, s, m)};
+                    *(uint4_t *)(keys + to * P::kKeyBytes + ((group + odd) * 32 + k_quad * 8) * 2) = out;
+                }
+            }
+            // what no row sees may be anything: its values are zeros (its scores are left out); so are the groups that are not
+            // finite, which the rows that see them get from `unsound`
+            uint32_t scales[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const int t = v_block * 4 + j;
+                const bool seen = (x.there >> (t / 16) & 1) && at + t <= tile.pos_high && at + t < limit && (a.window == 0 || at + t > tile.pos_low - a.window);
+                const uint32_t w = x.v_scales[j];
+                const bool bad = (w & 0x7C000000u) == 0x7C000000u || (w & 0x7C00u) == 0x7C00u;
+                if (seen && bad) {
+                    atomicOr(&unsound[into][t], 1u << (v_word / 4));
+                    unsound[into][P::kTile] = 1;
+                }
+                scales[j] = seen && !bad ? w : 0;
+            }
+            half2_t s[2], m[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                s[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x05040100u)) * half2_t{0.5f, 0.5f};
+                m[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x07060302u)) * half2_t{0.5f, 0.5f};
+            }
+            unsigned char *to = values + v_word * 8 * P::kValueBytes + (v_block / 4 * 16 + (v_block & 1) * 8 + (v_block >> 1 & 1) * 4) * 2;
+#pragma unroll
+            for (int piece = 0; piece < 2; piece++) {
+                const uint32_t select = piece ? 0x07060302u : 0x05040100u;
+                const uint32_t p0 = __builtin_amdgcn_perm(x.v[1], x.v[0], select), p1 = __builtin_amdgcn_perm(x.v[3], x.v[2], select);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const uint2_t out = {value2(i & 2 ? p0 >> 8 : p0, i & 1, s[0], m[0]), value2(i & 2 ? p1 >> 8 : p1, i & 1, s[1], m[1])};
+                    *(uint2_t *)(to + (piece * 4 + i) * P::kValueBytes) = out;
+                }
+            }
+        };
+
+        float16_t acc[G] = {};  // 32 dims each: transposed, this lane's row
+        float sum = 0, base = kEmpty;
+        uint32_t there = 0;
+        if (threadIdx.x < P::kTile + 1) unsound[0][threadIdx.x] = unsound[1][threadIdx.x] = 0;
+        __syncthreads();
+        if (first < end) {
+            const Raw x = load(first);
+            there = x.there;
+            store(x, first, 0);
+        }
+        __syncthreads();
+        for (int step = first; step < end; step++) {
+            const int now = (step - first) & 1, at = step * P::kTile;
+            const bool any_unsound = unsound[now][P::kTile];
+            Raw next;
+            const bool more = step + 1 < end;
+            if (more) next = load(step + 1);
+            // (a wave none of whose rows sees any of the tile leaves it out)
+            if (wave_rows > 0 && at <= wave_high && (a.window == 0 || at + P::kTile - 1 > wave_low - a.window)) {
+                const unsigned char *keys = stage[now], *values = stage[now] + P::kKeyTile;
+                const bool whole = there == (1u << (P::kTile / 16)) - 1 && at + P::kTile - 1 <= wave_low && at + P::kTile <= limit && (a.window == 0 || at > wave_high - a.window);
+                float16_t x[P::kSub];
+                float most = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < P::kSub; i++) {
+                    x[i] = float16_t{};
+#pragma unroll
+                    for (int k = 0; k < P::kDepths; k++)
+                        x[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(keys + (32 * i + l32) * P::kKeyBytes + (k * 16 + half * 8) * 2), q[k], x[i], 0, 0, 0);
+                    if (!whole) {
+                        asm volatile("");
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            const int t = at + 32 * i + 8 * (j >> 2) + 4 * half + (j & 3);
+                            const bool sees = t <= pos && t < limit && (a.window == 0 || t > pos - a.window) && (there >> (2 * i + (j >> 3)) & 1);
+                            x[i][j] = sees ? x[i][j] : -INFINITY;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < P::kSub; i++)
+#pragma unroll
+                    for (int j = 0; j < 16; j++) most = fmaxf(most, x[i][j]);
+                most = fmaxf(most, __shfl_xor(most, 32, kWave)) * to_log2;
+                if (__ballot(most - base > 14.0f)) {
+                    const float to = fmaxf(base, most - 6.0f), keep = __builtin_amdgcn_exp2f(base - to);
+                    base = to;
+                    sum *= keep;
+#pragma unroll
+                    for (int g = 0; g < G; g++) acc[g] *= keep;
+                }
+#pragma unroll
+                for (int i = 0; i < P::kSub; i++) {
+                    half8_t weights[2];
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], to_log2, -base));
+                        sum += w;
+                        weights[j >> 3][j & 7] = (_Float16)w;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int g = 0; g < G; g++)
+                            acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(values + (32 * g + l32) * P::kValueBytes + (32 * i + 16 * k + 8 * half) * 2), weights[k], acc[g], 0, 0, 0);
+                }
+                if (any_unsound) {
+                    for (int t = 0; t < P::kTile; t++) {
+                        const uint32_t groups = unsound[now][t];
+                        const bool sees = at + t <= pos && (a.window == 0 || at + t > pos - a.window);
+#pragma unroll
+                        for (int g = 0; g < G; g++)
+                            if (groups >> g & 1) acc[g] = sees ? float16_t{} + NAN : acc[g];
+                    }
+                }
+            }
+            if (more) {
+                there = next.there;
+                store(next, step + 1, now ^ 1);
+            }
+            __syncthreads();
+            if (any_unsound) {
+                if (threadIdx.x < P::kTile + 1) unsound[now][threadIdx.x] = 0;
+                __syncthreads();
+            }
+        }
+
+        sum += __shfl_xor(sum, 32, kWave);
+        if (real) {
+            const float inv = sum == 0.0f ? 0.0f : 2.0f / sum;  // (half of v was stored); nothing seen: 0
+            const Segments segments(a, plan, P::kRows, segments_at);
+            const size_t slot = ((size_t)kv * segments.per_head + worker + number) * P::kRows + in_tile;
+            if (!entire && half == 0) *(float2 *)(segments.bases + slot * 2) = make_float2(base, sum);
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int d = 32 * g + 8 * j + 4 * half;
+                    if (entire) {
+                        const uint2_t packed = {(uint32_t)f2h(acc[g][4 * j] * inv) | (uint32_t)f2h(acc[g][4 * j + 1] * inv) << 16,
+                                                (uint32_t)f2h(acc[g][4 * j + 2] * inv) | (uint32_t)f2h(acc[g][4 * j + 3] * inv) << 16};
+                        *(uint2_t *)(a.output + query * a.output_stride + (size_t)head * kDim + d) = packed;
+                    } else {
+                        *(float4_t *)(segments.sums + slot * kDim + d) =
+                            float4_t{acc[g][4 * j] * 2.0f, acc[g][4 * j + 1] * 2.0f, acc[g][4 * j + 2] * 2.0f, acc[g][4 * j + 3] * 2.0f};
+                    }
+                }
+        }
+        left -= count;
+        if (plan.alone || left <= 0) return;
+        offset = 0;
+        do {
+            if (++number >= numbers) return;
+            tile = RowTile(a, plan, number, P::kRows, P::kTile);
+        } while (tile.steps == 0);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- launches
+
+constexpr int kFewRows = 64;  // (query rows times heads of a kv head) that go the way of few rows
+
+int decode_rows(long long rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
+int decode_step(int rows) { return rows == 4 ? 64 : 32; }
+
+// What a call launches: for sequences of few rows, for sequences of many, or both.
+struct Plans {
+    bool few, many;
+    RowPlan few_plan, many_plan;
+    int few_rows;  // per tile
+    size_t few_bytes, many_bytes;
+};
+
+// Steps that a row tile may have, as far as the host knows.
+long long most_steps(const AttentionKv4Args &a, int step) {
+    long long reach = a.max_length;
+    if (a.window > 0 && (long long)a.window + a.max_query < reach) reach = (long long)a.window + a.max_query;
+    return (reach + step - 1) / step + 1;
 }
 
 template <int kDim>
-hipError_t launch_decode(const AttentionKv4Args &a, hipStream_t s) {
-    const DecodePlan plan = decode_plan(a);
-    switch (decode_rows(a)) {
-        case 4: return launch_decode_rows<kDim, 4>(a, plan, s);
-        case 8: return launch_decode_rows<kDim, 8>(a, plan, s);
-        default: return launch_decode_rows<kDim, 16>(a, plan, s);
+Plans plans_of(const AttentionKv4Args &a) {
+    using P = Prompt<kDim>;
+    const int kv = a.cache.n_kv_heads, cus = std::min(current_device_cus(), 256), heads = a.n_heads / kv;
+    const long long rows = (long long)a.max_query * heads;
+    Plans p{};
+    // One sequence, or as many rows as all sequences can have: no sequence is expected to be shorter than the others
+    const bool alike = a.batch.batch == 1 || (long long)a.batch.batch * a.max_query <= a.batch.n_tokens;
+    p.many = rows > kFewRows;
+    p.few = !p.many || !alike;
+    if (p.few) {
+        const long long most = std::min<long long>(rows, kFewRows);
+        p.few_rows = decode_rows(most);
+        p.few_plan = RowPlan{0, (int)((most + p.few_rows - 1) / p.few_rows), 1, 0, 0, p.many ? kFewRows + 1 : INT32_MAX};
+        p.few_plan.alone = most_steps(a, decode_step(p.few_rows)) <= kAloneSteps;
+        // two waves a SIMD
+        p.few_plan.workers = p.few_plan.alone ? a.batch.batch * p.few_plan.tiles : (8 * cus + kv - 1) / kv;
+        p.few_bytes = p.few_plan.alone ? 0 : (Segments::bytes(a, p.few_plan, p.few_rows) + 15) / 16 * 16;
+    }
+    if (p.many) {
+        p.many_plan = RowPlan{0, (int)((rows + P::kRows - 1) / P::kRows), 1, 0, p.few ? kFewRows + 1 : 0, INT32_MAX};
+        const long long tiles = (long long)a.batch.batch * p.many_plan.tiles;
+        // two workgroups a CU
+        p.many_plan.alone = tiles * kv >= 2 * cus || most_steps(a, P::kTile) <= 4;
+        p.many_plan.workers = p.many_plan.alone ? (int)tiles : (2 * cus + kv - 1) / kv;
+        p.many_plan.least = 4;
+        p.many_bytes = p.many_plan.alone ? 0 : Segments::bytes(a, p.many_plan, P::kRows);
+    }
+    return p;
+}
+
+dim3 worker_grid(const AttentionKv4Args &a, const RowPlan &plan) {
+    const int across = std::min(plan.workers, 32768);
+    return dim3((unsigned)a.cache.n_kv_heads, (unsigned)across, (unsigned)((plan.workers + across - 1) / across));
+}
+
+template <int kDim, int kRows, int kStep>
+hipError_t launch_join(const AttentionKv4Args &a, const RowPlan &plan, size_t segments_at, hipStream_t s) {
+    const unsigned tiles = (unsigned)(a.batch.batch * plan.tiles), kv = (unsigned)a.cache.n_kv_heads;
+    const size_t lds = 16 * (size_t)plan.workers;  // a weight per row and part, of which there are at most `workers`
+    if ((long long)tiles * kv * (kRows / 4) < current_device_cus())
+        attention_join_kernel<kDim, kRows, kStep, 8><<<dim3(tiles, kv, kRows / 4 * (kDim / 32)), kJoinThreads, lds, s>>>(a, plan, segments_at);
+    else
+        attention_join_kernel<kDim, kRows, kStep, kDim / 4><<<dim3(tiles, kv, kRows / 4), kJoinThreads, lds, s>>>(a, plan, segments_at);
+    return hipGetLastError();
+}
+
+template <int kDim, int kRows>
+hipError_t launch_few(const AttentionKv4Args &a, const RowPlan &plan, hipStream_t s) {
+    if (plan.alone) {
+        attention_decode_kernel<kDim, kRows, kAloneWaves><<<worker_grid(a, plan), kAloneWaves * kWave, 0, s>>>(a, plan);
+        return hipGetLastError();
+    }
+    attention_decode_kernel<kDim, kRows, 1><<<worker_grid(a, plan), kWave, 0, s>>>(a, plan);
+    if (hipError_t e = hipGetLastError()) return e;
+    return launch_join<kDim, kRows, Decode<kDim, kRows>::kStep>(a, plan, 0, s);
+}
+
+template <int kDim>
+hipError_t launch(const AttentionKv4Args &a, hipStream_t s) {
+    const Plans p = plans_of<kDim>(a);
+    if (p.many) {
+        attention_prompt_kernel<kDim><<<worker_grid(a, p.many_plan), Prompt<kDim>::kThreads, 0, s>>>(a, p.many_plan, p.few_bytes);
+        if (hipError_t e = hipGetLastError()) return e;
+        if (!p.many_plan.alone)
+            if (hipError_t e = launch_join<kDim, Prompt<kDim>::kRows, Prompt<kDim>::kTile>(a, p.many_plan, p.few_bytes, s)) return e;
+    }
+    if (!p.few) return hipSuccess;
+    switch (p.few_rows) {
+        case 4: return launch_few<kDim, 4>(a, p.few_plan, s);
+        case 8: return launch_few<kDim, 8>(a, p.few_plan, s);
+        default: return launch_few<kDim, 16>(a, p.few_plan, s);
     }
 }
 
 }  // namespace
 
 size_t attention_kv4_workspace(const AttentionKv4Args &a) {
-    const DecodePlan plan = decode_plan(a);
-    return plan.alone ? 0 : Segments::bytes(a, plan, decode_rows(a));
+    const Plans p = a.cache.head_dim == 64 ? plans_of<64>(a) : plans_of<128>(a);
+    return p.few_bytes + p.many_bytes;
 }
 
 hipError_t launch_attention_kv4(const AttentionKv4Args &a, hipStream_t s) {
-    return a.cache.head_dim == 64 ? launch_decode<64>(a, s) : launch_decode<128>(a, s);
+    return a.cache.head_dim == 64 ? launch<64>(a, s) : launch<128>(a, s);
 }
 
 }  // namespace tllm
