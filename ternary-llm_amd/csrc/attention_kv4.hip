@@ -761,20 +761,20 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Atte
 // again as all the rest. Half of k and v are stored: m + 15 s may be half a step of s above fp16's largest.
 // Transposed products (k q^T, v^T p^T) put a row's scores into one lane and its partner 32 lanes on, and p is then the next
 // product's operand as it lies, if v's positions are ordered like the result rows of the first product (8 b + 4 h + r).
-template <int kDim>
+template <int kDim, int kWaves_>
 struct Prompt {
     static constexpr int kGroups = kDim / kKvGroup, kWords = kDim / 8;
-    static constexpr int kTile = 8192 / kDim;  // 32 values of k and of v per thread
-    static constexpr int kWaves = 4, kThreads = kWaves * kWave, kRows = kWaves * 32;
+    static constexpr int kWaves = kWaves_, kThreads = kWaves * kWave, kRows = kWaves * 32;
+    static constexpr int kTile = 32 * kThreads / kDim;  // 32 values of k and of v per thread
     static constexpr int kKeyBytes = kDim * 2 + 16, kValueBytes = kTile * 2 + 16;  // rows in LDS, off the banks' period
     static constexpr int kKeyTile = kTile * kKeyBytes, kStage = kKeyTile + kDim * kValueBytes;
-    static constexpr int kSub = kTile / 32, kDepths = kDim / 16;
+    static constexpr int kChunk = 64, kSub = kChunk / 32, kDepths = kDim / 16;  // positions that a wave has scores of at once
 };
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
-template <int kDim>
-__global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const AttentionKv4Args a, const RowPlan plan, size_t segments_at) {
-    using P = Prompt<kDim>;
+template <int kDim, int kWaves>
+__global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(const AttentionKv4Args a, const RowPlan plan, size_t segments_at) {
+    using P = Prompt<kDim, kWaves>;
     constexpr int G = P::kGroups;
     __shared__ __align__(16) unsigned char stage[2][P::kStage];
     __shared__ uint32_t unsound[2][P::kTile + 1];  // groups of each position's value that are not finite; and whether any is
@@ -825,6 +825,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
             uint32_t k_scales[4];
             uint32_t there;  // bit i: positions 16 i .. 16 i + 15 have a page
         };
+        static_assert(P::kTile <= 512, "a bit per 16 positions");
         // thread: 32 values of a position's key (one depth quad of every group; kDim 64: two positions) and of four positions' values
         const int k_quad = threadIdx.x & 3, k_pos = threadIdx.x >> 2;
         const int v_block = threadIdx.x % (P::kTile / 4), v_word = threadIdx.x / (P::kTile / 4);
@@ -841,38 +842,50 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
                 const int index = (at + 16 * i) >> c.page_shift, page = __builtin_amdgcn_readlane(held, index - held_from);
                 x.there |= (uint32_t)(index < a.batch.width && page >= 0 && page < c.n_pages) << i;
             }
-            auto block_of = [&](int t) {
-                const int page = __shfl(held, ((at + t) >> c.page_shift) - held_from, kWave);
-                return (size_t)((x.there >> (t / 16) & 1 ? page : 0) * c.n_kv_heads + kv);
-            };
+            // (one page: the block is the same for all threads, and so are the bases)
+            const bool one_page = 1 << c.page_shift >= P::kTile;
+            const int page0 = __builtin_amdgcn_readlane(held, (at >> c.page_shift) - held_from);
+            const size_t block0 = (size_t)((x.there & 1 ? page0 : 0) * c.n_kv_heads + kv);
             const int slots = (1 << c.page_shift) - 1;
-            if constexpr (G == 4) {
-                const size_t b = block_of(k_pos);
-                const int slot = (at + k_pos) & slots;
-                x.k = *(const uint4_t *)(c.k_codes + b * code_words + (size_t)slot * P::kWords + k_quad * G);
+            auto fetch = [&](auto block_of, int first_slot) {
+                if constexpr (G == 4) {
+                    const size_t b = block_of(k_pos);
+                    const uint32_t slot = (uint32_t)(first_slot + k_pos) & slots;
+                    x.k = *(const uint4_t *)((const unsigned char *)(c.k_codes + b * code_words) + (slot * P::kWords + k_quad * G) * 4);
 #pragma unroll
-                for (int g = 0; g < 4; g++) x.k_scales[g] = c.k_scales[b * scale_words + ((size_t)g << c.page_shift) + slot];
-            } else {
+                    for (int g = 0; g < 4; g++) x.k_scales[g] = *(const uint32_t *)((const unsigned char *)(c.k_scales + b * scale_words + ((size_t)g << c.page_shift)) + slot * 4);
+                } else {
 #pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    const size_t b = block_of(k_pos + 64 * i);
-                    const int slot = (at + k_pos + 64 * i) & slots;
-                    const uint2_t two = *(const uint2_t *)(c.k_codes + b * code_words + (size_t)slot * P::kWords + k_quad * G);
-                    x.k[2 * i] = two[0];
-                    x.k[2 * i + 1] = two[1];
+                    for (int i = 0; i < 2; i++) {
+                        const size_t b = block_of(k_pos + P::kTile / 2 * i);
+                        const uint32_t slot = (uint32_t)(first_slot + k_pos + P::kTile / 2 * i) & slots;
+                        const uint2_t two = *(const uint2_t *)((const unsigned char *)(c.k_codes + b * code_words) + (slot * P::kWords + k_quad * G) * 4);
+                        x.k[2 * i] = two[0];
+                        x.k[2 * i + 1] = two[1];
 #pragma unroll
-                    for (int g = 0; g < 2; g++) x.k_scales[2 * i + g] = c.k_scales[b * scale_words + ((size_t)g << c.page_shift) + slot];
+                        for (int g = 0; g < 2; g++) x.k_scales[2 * i + g] = *(const uint32_t *)((const unsigned char *)(c.k_scales + b * scale_words + ((size_t)g << c.page_shift)) + slot * 4);
+                    }
                 }
+                const size_t b = block_of(v_block * 4);
+                const uint32_t slot = (uint32_t)(first_slot + v_block * 4) & slots;
+                x.v = *(const uint4_t *)((const unsigned char *)(c.v_codes + b * code_words) + (slot * P::kWords + v_word * 4) * 4);
+                x.v_scales = *(const uint4_t *)((const unsigned char *)(c.v_scales + b * scale_words) + (((uint32_t)(v_word / 4) << c.page_shift) + slot) * 4);
+            };
+            if (one_page) {
+                fetch([&](int) { return block0; }, at);
+            } else {
+                fetch([&](int t) {
+                    const int page = __shfl(held, ((at + t) >> c.page_shift) - held_from, kWave);
+                    return (size_t)((x.there >> (t / 16) & 1 ? page : 0) * c.n_kv_heads + kv);
+                }, at);
             }
-            const size_t b = block_of(v_block * 4);
-            const int slot = (at + v_block * 4) & slots;
-            x.v = *(const uint4_t *)(c.v_codes + b * code_words + (size_t)slot * P::kWords + v_word * 4);
-            x.v_scales = *(const uint4_t *)(c.v_scales + b * scale_words + ((size_t)(v_word / 4) << c.page_shift) + slot);
             return x;
         };
         // codes 1024 + c (64 + c from bits 4-7) less the rest, times s / 2, plus m / 2
-        auto value2 = [](uint32_t field, bool odd, half2_t s, half2_t m) {
-            const half2_t code = __builtin_bit_cast(half2_t, odd ? (field & kOddCodes) | 0x54005400u : (field & kEvenCodes) | 0x64006400u) - (odd ? half2_t{64, 64} : half2_t{1024, 1024});
+        uint32_t even_bits = 0x64006400u, odd_bits = 0x54005400u;  // (in registers: two constants make two instructions)
+        asm("" : "+v"(even_bits), "+v"(odd_bits));
+        auto value2 = [&](uint32_t field, bool odd, half2_t s, half2_t m) {
+            const half2_t code = __builtin_bit_cast(half2_t, odd ? (field & kOddCodes) | odd_bits : (field & kEvenCodes) | even_bits) - (odd ? half2_t{64, 64} : half2_t{1024, 1024});
             return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, s, m));
         };
         auto store = [&](const Raw &x, int step, int into) {
@@ -881,7 +894,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
 #pragma unroll
             for (int pair = 0; pair < 2; pair++) {
                 const uint32_t w0 = x.k[2 * pair], w1 = x.k[2 * pair + 1];
-                const int to = G == 4 ? k_pos : k_pos + 64 * pair, group = G == 4 ? 2 * pair : 0;
+                const int to = G == 4 ? k_pos : k_pos + P::kTile / 2 * pair, group = G == 4 ? 2 * pair : 0;
 #pragma unroll
                 for (int odd = 0; odd < 2; odd++) {
                     const half2_t both = __builtin_bit_cast(half2_t, x.k_scales[2 * pair + odd]) * half2_t{0.5f, 0.5f};
@@ -927,7 +940,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
         float16_t acc[G] = {};  // 32 dims each: transposed, this lane's row
         float sum = 0, base = kEmpty;
         uint32_t there = 0;
-        if (threadIdx.x < P::kTile + 1) unsound[0][threadIdx.x] = unsound[1][threadIdx.x] = 0;
+        for (int t = threadIdx.x; t <= P::kTile; t += P::kThreads) unsound[0][t] = unsound[1][t] = 0;
         __syncthreads();
         if (first < end) {
             const Raw x = load(first);
@@ -941,10 +954,15 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
             Raw next;
             const bool more = step + 1 < end;
             if (more) next = load(step + 1);
-            // (a wave none of whose rows sees any of the tile leaves it out)
-            if (wave_rows > 0 && at <= wave_high && (a.window == 0 || at + P::kTile - 1 > wave_low - a.window)) {
-                const unsigned char *keys = stage[now], *values = stage[now] + P::kKeyTile;
-                const bool whole = there == (1u << (P::kTile / 16)) - 1 && at + P::kTile - 1 <= wave_low && at + P::kTile <= limit && (a.window == 0 || at > wave_high - a.window);
+#pragma unroll 1
+            for (int chunk = 0; chunk < P::kTile; chunk += P::kChunk) {
+                const int from = at + chunk;
+                // (a wave none of whose rows sees any of the positions leaves them out)
+                if (wave_rows <= 0 || from > wave_high || (a.window > 0 && from + P::kChunk - 1 <= wave_low - a.window)) continue;
+                const unsigned char *keys = stage[now] + (chunk + l32) * P::kKeyBytes + half * 16;
+                const unsigned char *values = stage[now] + P::kKeyTile + l32 * P::kValueBytes + (chunk + half * 8) * 2;
+                const uint32_t pages = there >> (chunk / 16) & ((1u << (P::kChunk / 16)) - 1);
+                const bool whole = pages == (1u << (P::kChunk / 16)) - 1 && from + P::kChunk - 1 <= wave_low && from + P::kChunk <= limit && (a.window == 0 || from > wave_high - a.window);
                 float16_t x[P::kSub];
                 float most = -INFINITY;
 #pragma unroll
@@ -952,16 +970,18 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
                     x[i] = float16_t{};
 #pragma unroll
                     for (int k = 0; k < P::kDepths; k++)
-                        x[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(keys + (32 * i + l32) * P::kKeyBytes + (k * 16 + half * 8) * 2), q[k], x[i], 0, 0, 0);
-                    if (!whole) {
-                        asm volatile("");
+                        x[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(keys + 32 * i * P::kKeyBytes + k * 32), q[k], x[i], 0, 0, 0);
+                }
+                if (!whole) {
+                    asm volatile("");
+#pragma unroll
+                    for (int i = 0; i < P::kSub; i++)
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            const int t = at + 32 * i + 8 * (j >> 2) + 4 * half + (j & 3);
-                            const bool sees = t <= pos && t < limit && (a.window == 0 || t > pos - a.window) && (there >> (2 * i + (j >> 3)) & 1);
+                            const int t = from + 32 * i + 8 * (j >> 2) + 4 * half + (j & 3);
+                            const bool sees = t <= pos && t < limit && (a.window == 0 || t > pos - a.window) && (pages >> (2 * i + (j >> 3)) & 1);
                             x[i][j] = sees ? x[i][j] : -INFINITY;
                         }
-                    }
                 }
 #pragma unroll
                 for (int i = 0; i < P::kSub; i++)
@@ -979,19 +999,18 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
                 for (int i = 0; i < P::kSub; i++) {
                     half8_t weights[2];
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], to_log2, -base));
-                        sum += w;
-                        weights[j >> 3][j & 7] = (_Float16)w;
-                    }
+                    for (int j = 0; j < 16; j++) weights[j >> 3][j & 7] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[i][j], to_log2, -base));
+#pragma unroll
+                    for (int j = 0; j < 16; j += 2)  // (of the rounded weights, which is what the values are multiplied with)
+                        sum = __builtin_amdgcn_fdot2(half2_t{weights[j >> 3][j & 7], weights[j >> 3][(j & 7) + 1]}, half2_t{1, 1}, sum, false);
 #pragma unroll
                     for (int k = 0; k < 2; k++)
 #pragma unroll
                         for (int g = 0; g < G; g++)
-                            acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(values + (32 * g + l32) * P::kValueBytes + (32 * i + 16 * k + 8 * half) * 2), weights[k], acc[g], 0, 0, 0);
+                            acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(values + 32 * g * P::kValueBytes + (32 * i + 16 * k) * 2), weights[k], acc[g], 0, 0, 0);
                 }
                 if (any_unsound) {
-                    for (int t = 0; t < P::kTile; t++) {
+                    for (int t = chunk; t < chunk + P::kChunk; t++) {
                         const uint32_t groups = unsound[now][t];
                         const bool sees = at + t <= pos && (a.window == 0 || at + t > pos - a.window);
 #pragma unroll
@@ -1006,7 +1025,7 @@ __global__ __launch_bounds__(256, 2) void attention_prompt_kernel(const Attentio
             }
             __syncthreads();
             if (any_unsound) {
-                if (threadIdx.x < P::kTile + 1) unsound[now][threadIdx.x] = 0;
+                for (int t = threadIdx.x; t <= P::kTile; t += P::kThreads) unsound[now][t] = 0;
                 __syncthreads();
             }
         }
@@ -1054,6 +1073,7 @@ struct Plans {
     bool few, many;
     RowPlan few_plan, many_plan;
     int few_rows;  // per tile
+    int many_waves;
     size_t few_bytes, many_bytes;
 };
 
@@ -1064,9 +1084,12 @@ long long most_steps(const AttentionKv4Args &a, int step) {
     return (reach + step - 1) / step + 1;
 }
 
+#ifndef PW
+#define PW 8
+#endif
+constexpr int kPromptWaves = PW;
 template <int kDim>
 Plans plans_of(const AttentionKv4Args &a) {
-    using P = Prompt<kDim>;
     const int kv = a.cache.n_kv_heads, cus = std::min(current_device_cus(), 256), heads = a.n_heads / kv;
     const long long rows = (long long)a.max_query * heads;
     Plans p{};
@@ -1084,13 +1107,15 @@ Plans plans_of(const AttentionKv4Args &a) {
         p.few_bytes = p.few_plan.alone ? 0 : (Segments::bytes(a, p.few_plan, p.few_rows) + 15) / 16 * 16;
     }
     if (p.many) {
-        p.many_plan = RowPlan{0, (int)((rows + P::kRows - 1) / P::kRows), 1, 0, p.few ? kFewRows + 1 : 0, INT32_MAX};
+        p.many_waves = kPromptWaves;
+        const int tile_rows = p.many_waves * 32, step = 2048 * p.many_waves / kDim;
+        p.many_plan = RowPlan{0, (int)((rows + tile_rows - 1) / tile_rows), 1, 0, p.few ? kFewRows + 1 : 0, INT32_MAX};
         const long long tiles = (long long)a.batch.batch * p.many_plan.tiles;
-        // two workgroups a CU
-        p.many_plan.alone = tiles * kv >= 2 * cus || most_steps(a, P::kTile) <= 4;
-        p.many_plan.workers = p.many_plan.alone ? (int)tiles : (2 * cus + kv - 1) / kv;
-        p.many_plan.least = 4;
-        p.many_bytes = p.many_plan.alone ? 0 : Segments::bytes(a, p.many_plan, P::kRows);
+        const int slots = 8 / p.many_waves * cus;  // two waves a SIMD
+        p.many_plan.alone = tiles * kv >= slots || most_steps(a, step) <= 4;
+        p.many_plan.workers = p.many_plan.alone ? (int)tiles : (slots + kv - 1) / kv;
+        p.many_plan.least = 2;
+        p.many_bytes = p.many_plan.alone ? 0 : Segments::bytes(a, p.many_plan, tile_rows);
     }
     return p;
 }
@@ -1122,15 +1147,19 @@ hipError_t launch_few(const AttentionKv4Args &a, const RowPlan &plan, hipStream_
     return launch_join<kDim, kRows, Decode<kDim, kRows>::kStep>(a, plan, 0, s);
 }
 
+template <int kDim, int kWaves>
+hipError_t launch_many(const AttentionKv4Args &a, const RowPlan &plan, size_t segments_at, hipStream_t s) {
+    using P = Prompt<kDim, kWaves>;
+    attention_prompt_kernel<kDim, kWaves><<<worker_grid(a, plan), P::kThreads, 0, s>>>(a, plan, segments_at);
+    if (hipError_t e = hipGetLastError()) return e;
+    return plan.alone ? hipSuccess : launch_join<kDim, P::kRows, P::kTile>(a, plan, segments_at, s);
+}
+
 template <int kDim>
 hipError_t launch(const AttentionKv4Args &a, hipStream_t s) {
     const Plans p = plans_of<kDim>(a);
-    if (p.many) {
-        attention_prompt_kernel<kDim><<<worker_grid(a, p.many_plan), Prompt<kDim>::kThreads, 0, s>>>(a, p.many_plan, p.few_bytes);
-        if (hipError_t e = hipGetLastError()) return e;
-        if (!p.many_plan.alone)
-            if (hipError_t e = launch_join<kDim, Prompt<kDim>::kRows, Prompt<kDim>::kTile>(a, p.many_plan, p.few_bytes, s)) return e;
-    }
+    if (p.many)
+        if (hipError_t e = launch_many<kDim, kPromptWaves>(a, p.many_plan, p.few_bytes, s)) return e;
     if (!p.few) return hipSuccess;
     switch (p.few_rows) {
         case 4: return launch_few<kDim, 4>(a, p.few_plan, s);
