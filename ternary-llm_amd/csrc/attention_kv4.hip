@@ -759,6 +759,8 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Atte
 // while the tile before is worked on. k and v are rounded to fp16 there, and p for the second product: three roundings of
 // 2^-12 (root mean square) next to the result's own; exact codes and two pieces of p, as for few rows, would cost as much
 // again as all the rest. Half of k and v are stored: m + 15 s may be half a step of s above fp16's largest.
+// v's rows of positions are stored with their 16-byte pieces exchanged by the row's eight (an exclusive or): the writes of a wave,
+// eight rows apart, would otherwise meet in two banks.
 // Transposed products (k q^T, v^T p^T) put a row's scores into one lane and its partner 32 lanes on, and p is then the next
 // product's operand as it lies, if v's positions are ordered like the result rows of the first product (8 b + 4 h + r).
 template <int kDim, int kWaves_>
@@ -797,7 +799,8 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
     }
     const int limit = position_limit(a);
     const size_t code_words = kv4_code_words(1 << c.page_shift, kDim), scale_words = kv4_scale_words(1 << c.page_shift, kDim);
-    const float to_log2 = fabsf(a.scale) * (2.0f * 1.44269504088896f);  // (the sign is the row operand's)
+    // (the sign is the row operand's; a scale of 0 makes that 0, so that what is left out can stay at minus infinity)
+    const float to_log2 = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * (2.0f * 1.44269504088896f);
 
     while (true) {
         const int count = min(tile.steps - offset, left);
@@ -815,6 +818,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
         for (int k = 0; k < P::kDepths; k++) {
             q[k] = real ? *(const half8_t *)(a.q + query * a.q_stride + (size_t)head * kDim + k * 16 + half * 8) : half8_t{};
             if (a.scale < 0) q[k] = -q[k];
+            if (a.scale == 0) q[k] = half8_t{};
         }
         const int wave_rows = min(32, tile.rows_left - wave * 32);  // (none: the wave only helps with the tiles)
         const int wave_low = tile.pos0 + (tile.first_row + wave * 32) / heads, wave_high = tile.pos0 + (tile.first_row + wave * 32 + max(wave_rows, 1) - 1) / heads;
@@ -825,10 +829,15 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
             uint32_t k_scales[4];
             uint32_t there;  // bit i: positions 16 i .. 16 i + 15 have a page
         };
-        static_assert(P::kTile <= 512, "a bit per 16 positions");
-        // thread: 32 values of a position's key (one depth quad of every group; kDim 64: two positions) and of four positions' values
-        const int k_quad = threadIdx.x & 3, k_pos = threadIdx.x >> 2;
-        const int v_block = threadIdx.x % (P::kTile / 4), v_word = threadIdx.x / (P::kTile / 4);
+        static_assert(P::kTile / 16 == kWaves * (4 / G) && P::kTile <= 512, "a wave takes 16 positions (kDim 64: two times 16); a bit each");
+        // A wave takes 16 whole positions of the tile, so that their page is the same for all its lanes: of the keys, a lane has
+        // one depth quad of every group of a position, of the values a word of four positions (kDim 64: half the lanes each 16).
+        constexpr int kBlocks = 4 / G;
+        const int k_quad = lane & 3, k_pos = lane >> 2;
+        const int v_block = lane & 3, v_word = G == 4 ? lane >> 2 : lane >> 2 & 7, v_part = G == 4 ? 0 : lane >> 5;
+        const uint32_t k_offset = (uint32_t)(k_pos * P::kWords + k_quad * G) * 4, ks_offset = (uint32_t)k_pos * 4;
+        const uint32_t v_offset = (uint32_t)(v_block * 4 * P::kWords + v_word * 4) * 4, vs_offset = (((uint32_t)(v_word / 4) << c.page_shift) + v_block * 4) * 4;
+        const int slots = (1 << c.page_shift) - 1;
         auto load = [&](int step) {
             Raw x;
             const int at = step * P::kTile, last = (at + P::kTile - 16) >> c.page_shift;
@@ -836,49 +845,30 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
                 held_from = at >> c.page_shift;
                 held = table[min(held_from + lane, a.batch.width - 1)];
             }
-            x.there = 0;
+            const int index = (at + 16 * lane) >> c.page_shift, its = __shfl(held, min(index - held_from, kWave - 1), kWave);
+            x.there = (uint32_t)__ballot(lane < P::kTile / 16 && index < a.batch.width && its >= 0 && its < c.n_pages);
+            const unsigned char *v_at[2], *vs_at[2];
 #pragma unroll
-            for (int i = 0; i < P::kTile / 16; i++) {
-                const int index = (at + 16 * i) >> c.page_shift, page = __builtin_amdgcn_readlane(held, index - held_from);
-                x.there |= (uint32_t)(index < a.batch.width && page >= 0 && page < c.n_pages) << i;
-            }
-            // (one page: the block is the same for all threads, and so are the bases)
-            const bool one_page = 1 << c.page_shift >= P::kTile;
-            const int page0 = __builtin_amdgcn_readlane(held, (at >> c.page_shift) - held_from);
-            const size_t block0 = (size_t)((x.there & 1 ? page0 : 0) * c.n_kv_heads + kv);
-            const int slots = (1 << c.page_shift) - 1;
-            auto fetch = [&](auto block_of, int first_slot) {
+            for (int i = 0; i < kBlocks; i++) {
+                const int part = wave + kWaves * i, from = at + 16 * part;
+                const int page = x.there >> part & 1 ? __builtin_amdgcn_readlane(held, (from >> c.page_shift) - held_from) : 0;
+                const size_t block = (size_t)(page * c.n_kv_heads + kv), slot = from & slots;
+                const unsigned char *k_at = (const unsigned char *)(c.k_codes + block * code_words + slot * P::kWords) + k_offset;
+                const unsigned char *ks_at = (const unsigned char *)(c.k_scales + block * scale_words + slot) + ks_offset;
+                v_at[i] = (const unsigned char *)(c.v_codes + block * code_words + slot * P::kWords) + v_offset;
+                vs_at[i] = (const unsigned char *)(c.v_scales + block * scale_words + slot) + vs_offset;
                 if constexpr (G == 4) {
-                    const size_t b = block_of(k_pos);
-                    const uint32_t slot = (uint32_t)(first_slot + k_pos) & slots;
-                    x.k = *(const uint4_t *)((const unsigned char *)(c.k_codes + b * code_words) + (slot * P::kWords + k_quad * G) * 4);
-#pragma unroll
-                    for (int g = 0; g < 4; g++) x.k_scales[g] = *(const uint32_t *)((const unsigned char *)(c.k_scales + b * scale_words + ((size_t)g << c.page_shift)) + slot * 4);
+                    x.k = *(const uint4_t *)k_at;
                 } else {
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {
-                        const size_t b = block_of(k_pos + P::kTile / 2 * i);
-                        const uint32_t slot = (uint32_t)(first_slot + k_pos + P::kTile / 2 * i) & slots;
-                        const uint2_t two = *(const uint2_t *)((const unsigned char *)(c.k_codes + b * code_words) + (slot * P::kWords + k_quad * G) * 4);
-                        x.k[2 * i] = two[0];
-                        x.k[2 * i + 1] = two[1];
-#pragma unroll
-                        for (int g = 0; g < 2; g++) x.k_scales[2 * i + g] = *(const uint32_t *)((const unsigned char *)(c.k_scales + b * scale_words + ((size_t)g << c.page_shift)) + slot * 4);
-                    }
+                    const uint2_t two = *(const uint2_t *)k_at;
+                    x.k[2 * i] = two[0];
+                    x.k[2 * i + 1] = two[1];
                 }
-                const size_t b = block_of(v_block * 4);
-                const uint32_t slot = (uint32_t)(first_slot + v_block * 4) & slots;
-                x.v = *(const uint4_t *)((const unsigned char *)(c.v_codes + b * code_words) + (slot * P::kWords + v_word * 4) * 4);
-                x.v_scales = *(const uint4_t *)((const unsigned char *)(c.v_scales + b * scale_words) + (((uint32_t)(v_word / 4) << c.page_shift) + slot) * 4);
-            };
-            if (one_page) {
-                fetch([&](int) { return block0; }, at);
-            } else {
-                fetch([&](int t) {
-                    const int page = __shfl(held, ((at + t) >> c.page_shift) - held_from, kWave);
-                    return (size_t)((x.there >> (t / 16) & 1 ? page : 0) * c.n_kv_heads + kv);
-                }, at);
+#pragma unroll
+                for (int g = 0; g < G; g++) x.k_scales[G * i + g] = *(const uint32_t *)(ks_at + ((size_t)g << (c.page_shift + 2)));
             }
+            x.v = *(const uint4_t *)(kBlocks == 2 && v_part ? v_at[1] : v_at[0]);
+            x.v_scales = *(const uint4_t *)(kBlocks == 2 && v_part ? vs_at[1] : vs_at[0]);
             return x;
         };
         // codes 1024 + c (64 + c from bits 4-7) less the rest, times s / 2, plus m / 2
@@ -894,7 +884,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
 #pragma unroll
             for (int pair = 0; pair < 2; pair++) {
                 const uint32_t w0 = x.k[2 * pair], w1 = x.k[2 * pair + 1];
-                const int to = G == 4 ? k_pos : k_pos + P::kTile / 2 * pair, group = G == 4 ? 2 * pair : 0;
+                const int to = 16 * (wave + (G == 4 ? 0 : kWaves * pair)) + k_pos, group = G == 4 ? 2 * pair : 0;
 #pragma unroll
                 for (int odd = 0; odd < 2; odd++) {
                     const half2_t both = __builtin_bit_cast(half2_t, x.k_scales[2 * pair + odd]) * half2_t{0.5f, 0.5f};
@@ -905,18 +895,29 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
             }
             // what no row sees may be anything: its values are zeros (its scores are left out); so are the groups that are not
             // finite, which the rows that see them get from `unsound`
-            uint32_t scales[4];
+            const int part = wave + kWaves * v_part, from = at + 16 * part + v_block * 4;
+            uint32_t scales[4], odd_one = 0;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int t = v_block * 4 + j;
-                const bool seen = (x.there >> (t / 16) & 1) && at + t <= tile.pos_high && at + t < limit && (a.window == 0 || at + t > tile.pos_low - a.window);
-                const uint32_t w = x.v_scales[j];
-                const bool bad = (w & 0x7C000000u) == 0x7C000000u || (w & 0x7C00u) == 0x7C00u;
-                if (seen && bad) {
-                    atomicOr(&unsound[into][t], 1u << (v_word / 4));
-                    unsound[into][P::kTile] = 1;
+                scales[j] = x.v_scales[j];
+                odd_one |= (scales[j] & 0x7C007C00u) + 0x04000400u;  // bits 15 and 31: an exponent is all ones
+            }
+            // (positions of this step that all lie where some row sees them: all but the ends)
+            const bool inside = x.there == (uint32_t)((1ull << (P::kTile / 16)) - 1) && at + P::kTile - 1 <= min(tile.pos_high, limit - 1) && (a.window == 0 || at > tile.pos_low - a.window);
+            if (!inside || __ballot(odd_one & 0x80008000u)) {
+                asm volatile("");
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int t = from + j;
+                    const bool seen = (x.there >> part & 1) && t <= tile.pos_high && t < limit && (a.window == 0 || t > tile.pos_low - a.window);
+                    const uint32_t w = scales[j];
+                    const bool bad = ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                    if (seen && bad) {
+                        atomicOr(&unsound[into][t - at], 1u << (v_word / 4));
+                        unsound[into][P::kTile] = 1;
+                    }
+                    scales[j] = seen && !bad ? w : 0;
                 }
-                scales[j] = seen && !bad ? w : 0;
             }
             half2_t s[2], m[2];
 #pragma unroll
@@ -924,7 +925,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
                 s[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x05040100u)) * half2_t{0.5f, 0.5f};
                 m[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x07060302u)) * half2_t{0.5f, 0.5f};
             }
-            unsigned char *to = values + v_word * 8 * P::kValueBytes + (v_block / 4 * 16 + (v_block & 1) * 8 + (v_block >> 1 & 1) * 4) * 2;
+            unsigned char *to = values + v_word * 8 * P::kValueBytes + ((part * 32 + (v_block & 1) * 16) ^ (v_word & 15) << 4) + (v_block >> 1) * 8;
 #pragma unroll
             for (int piece = 0; piece < 2; piece++) {
                 const uint32_t select = piece ? 0x07060302u : 0x05040100u;
@@ -942,25 +943,33 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
         uint32_t there = 0;
         for (int t = threadIdx.x; t <= P::kTile; t += P::kThreads) unsound[0][t] = unsound[1][t] = 0;
         __syncthreads();
+        Raw next;
         if (first < end) {
-            const Raw x = load(first);
-            there = x.there;
-            store(x, first, 0);
+            next = load(first);
+            there = next.there;
+            store(next, first, 0);
+            if (first + 1 < end) next = load(first + 1);
         }
         __syncthreads();
         for (int step = first; step < end; step++) {
             const int now = (step - first) & 1, at = step * P::kTile;
             const bool any_unsound = unsound[now][P::kTile];
-            Raw next;
-            const bool more = step + 1 < end;
-            if (more) next = load(step + 1);
+            uint32_t then = 0;
+            auto prepare = [&] {
+                if (step + 1 >= end) return;
+                then = next.there;
+                store(next, step + 1, now ^ 1);
+                if (step + 2 < end) next = load(step + 2);
+            };
+            // (the two waves of a SIMD begin a tile with different work: one uses the vector pipe while the other multiplies)
+            if (wave >= kWaves / 2) prepare();
 #pragma unroll 1
             for (int chunk = 0; chunk < P::kTile; chunk += P::kChunk) {
                 const int from = at + chunk;
                 // (a wave none of whose rows sees any of the positions leaves them out)
                 if (wave_rows <= 0 || from > wave_high || (a.window > 0 && from + P::kChunk - 1 <= wave_low - a.window)) continue;
                 const unsigned char *keys = stage[now] + (chunk + l32) * P::kKeyBytes + half * 16;
-                const unsigned char *values = stage[now] + P::kKeyTile + l32 * P::kValueBytes + (chunk + half * 8) * 2;
+                const unsigned char *values = stage[now] + P::kKeyTile + l32 * P::kValueBytes;
                 const uint32_t pages = there >> (chunk / 16) & ((1u << (P::kChunk / 16)) - 1);
                 const bool whole = pages == (1u << (P::kChunk / 16)) - 1 && from + P::kChunk - 1 <= wave_low && from + P::kChunk <= limit && (a.window == 0 || from > wave_high - a.window);
                 float16_t x[P::kSub];
@@ -1007,7 +1016,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
                     for (int k = 0; k < 2; k++)
 #pragma unroll
                         for (int g = 0; g < G; g++)
-                            acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(values + 32 * g * P::kValueBytes + (32 * i + 16 * k) * 2), weights[k], acc[g], 0, 0, 0);
+                            acc[g] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const half8_t *)(values + 32 * g * P::kValueBytes + ((chunk * 2 + (32 * i + 16 * k) * 2 + half * 16) ^ ((4 * g + (l32 >> 3)) & 15) << 4)), weights[k], acc[g], 0, 0, 0);
                 }
                 if (any_unsound) {
                     for (int t = chunk; t < chunk + P::kChunk; t++) {
@@ -1019,10 +1028,8 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
                     }
                 }
             }
-            if (more) {
-                there = next.there;
-                store(next, step + 1, now ^ 1);
-            }
+            if (wave < kWaves / 2) prepare();
+            there = then;
             __syncthreads();
             if (any_unsound) {
                 for (int t = threadIdx.x; t <= P::kTile; t += P::kThreads) unsound[now][t] = 0;
