@@ -1091,10 +1091,7 @@ long long most_steps(const AttentionKv4Args &a, int step) {
     return (reach + step - 1) / step + 1;
 }
 
-#ifndef PW
-#define PW 8
-#endif
-constexpr int kPromptWaves = PW;
+constexpr int kPromptWaves = 8;
 template <int kDim>
 Plans plans_of(const AttentionKv4Args &a) {
     const int kv = a.cache.n_kv_heads, cus = std::min(current_device_cus(), 256), heads = a.n_heads / kv;
