@@ -6,6 +6,7 @@ ternary_gemm. Mask tensors are int32 (the uint32 bit patterns), fp16 tensors are
 torch.float16. torch is used for device memory and streams only.
 """
 import ctypes as C
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -327,40 +328,41 @@ def _want(cond, text):
 
 def _rows(t, name, heads=None):
     """A tensor of rows [n, heads, dim]: fp16, heads next to each other; returns its row stride in elements."""
-    _want(t.dim() == 3 and t.dtype == _float16(), f"{name} must be fp16 [rows, heads, dim]")
-    n, h, d = t.shape
-    stride = t.stride()
-    _want((stride[2] == 1 or d == 1) and (stride[1] == d or h == 1), f"the heads of a row of {name} must lie next to each other")
-    _want(heads is None or h == heads, f"{name} has {h} heads, {heads} are expected")
+    if t.dim() != 3 or t.dtype != _torch().float16:
+        raise ValueError(f"{name} must be fp16 [rows, heads, dim]")
+    (n, h, d), stride = t.shape, t.stride()
+    if not ((stride[2] == 1 or d == 1) and (stride[1] == d or h == 1)):
+        raise ValueError(f"the heads of a row of {name} must lie next to each other")
+    if heads is not None and h != heads:
+        raise ValueError(f"{name} has {h} heads, {heads} are expected")
     return stride[0] if n > 1 else h * d
 
 
-def _float16():
+@functools.lru_cache(maxsize=None)
+def _torch():
     import torch
-    return torch.float16
+    return torch
 
 
-class _on:
-    """Launches go to the device of the tensors: makes it the current one if it is not (the library launches on the
-    current device) and gives the stream to use. A stream that is given must belong to that device."""
-
-    def __init__(self, stream, first, *others):
-        import torch
-        device = first.device
-        _want(first.is_cuda and all(t.device == device for t in others), "the tensors must lie on one GPU")
-        _want(stream is None or stream.device == device, "the stream belongs to another device than the tensors")
-        self.stream = torch.cuda.current_stream(device) if stream is None else stream
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return C.c_void_p(self.stream.cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _launch(stream, tensors, call):
+    """call(stream handle) with the tensors' device as the current one (the library launches on the current device). A stream
+    that is given must belong to that device."""
+    cuda = _torch().cuda
+    device = tensors[0].get_device()
+    for t in tensors:
+        if device < 0 or t.get_device() != device:
+            raise ValueError("the tensors must lie on one GPU")
+    if stream is None:
+        stream = cuda.current_stream(device)
+    elif stream.device_index != device:
+        raise ValueError("the stream belongs to another device than the tensors")
+    if device == cuda.current_device():
+        code = call(stream.cuda_stream)
+    else:
+        with cuda.device(device):
+            code = call(stream.cuda_stream)
+    if code != 0:
+        check(code)
 
 
 def rotary(q, k, q_out, k_out, positions, rotary_dim, theta, layout="interleaved", scaling="none", factor=1.0, original_length=8192,
@@ -385,33 +387,28 @@ def rotary(q, k, q_out, k_out, positions, rotary_dim, theta, layout="interleaved
         high_turns = 32.0 if scaling == "yarn" else 4.0
     config = _RotaryConfig(rotary_dim, ROTARY_LAYOUTS[layout], ROTARY_SCALINGS[scaling], original_length, theta, factor, low_turns,
                            high_turns, magnitude)
-    others = (q_out, positions) if k is None else (q_out, positions, k, k_out)
-    with _on(stream, q, *others) as s:
-        check(lib().tllm_rotary_f16(_ptr(q), _ptr(k), _ptr(q_out), _ptr(k_out), *strides, _ptr(positions), n, heads, kv_heads, dim,
-                                    config, s))
+    tensors = (q, q_out, positions) if k is None else (q, q_out, positions, k, k_out)
+    pointers = [None if t is None else t.data_ptr() for t in (q, k, q_out, k_out)]
+    _launch(stream, tensors, lambda s: lib().tllm_rotary_f16(*pointers, *strides, positions.data_ptr(), n, heads, kv_heads, dim, config, s))
 
 
 def _is_int32(t):
-    import torch
-    return t.dtype == torch.int32 and t.is_contiguous()
+    return t.dtype == _torch().int32 and t.is_contiguous()
 
 
 def _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n_tokens):
     """The two structs of a call from its tensors."""
     pages, heads, page, words = k_codes.shape
-    dim = words * 8
     _want(_is_int32(k_codes) and _is_int32(v_codes) and v_codes.shape == (pages, heads, page // 4, words, 4),
           "codes must be contiguous int32: k [pages, heads, page, dim / 8], v [pages, heads, page / 4, dim / 8, 4]")
-    shape = (pages, heads, dim // 32, page, 2)
-    half = _float16()
-    _want(k_scales.shape == shape and v_scales.shape == shape and k_scales.dtype == half and v_scales.dtype == half
+    half, shape = _torch().float16, (pages, heads, words // 4, page, 2)
+    _want(k_scales.dtype == half and v_scales.dtype == half and k_scales.shape == shape and v_scales.shape == shape
           and k_scales.is_contiguous() and v_scales.is_contiguous(), "scales must be contiguous fp16 [pages, heads, dim / 32, page, 2]")
-    batch, = lengths.shape
-    _want(_is_int32(query_starts) and _is_int32(lengths) and _is_int32(page_table) and query_starts.shape == (batch + 1,)
-          and page_table.dim() == 2 and page_table.shape[0] == batch,
+    (batch,), (rows, width) = lengths.shape, page_table.shape
+    _want(rows == batch and query_starts.shape == (batch + 1,) and _is_int32(query_starts) and _is_int32(lengths) and _is_int32(page_table),
           "query_starts [batch + 1], lengths [batch] and page_table [batch, width] must be contiguous int32")
-    return (_Kv4Cache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), pages, page, heads, dim),
-            _Kv4Batch(query_starts.data_ptr(), lengths.data_ptr(), page_table.data_ptr(), batch, n_tokens, page_table.shape[1]))
+    return (_Kv4Cache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), pages, page, heads, words * 8),
+            _Kv4Batch(query_starts.data_ptr(), lengths.data_ptr(), page_table.data_ptr(), batch, n_tokens, width))
 
 
 def kv4_cache(n_pages, page_size, n_kv_heads, head_dim, device="cuda"):
@@ -430,8 +427,8 @@ def kv4_append(k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths
     cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, k.shape[0])
     ks, vs = _rows(k, "k", cache.n_kv_heads), _rows(v, "v", cache.n_kv_heads)
     _want(k.shape == v.shape and k.shape[2] == cache.head_dim, "k and v must be [rows, kv_heads, dim] of the cache")
-    with _on(stream, k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table) as s:
-        check(lib().tllm_kv4_append_f16(_ptr(k), _ptr(v), ks, vs, cache, batch, s))
+    _launch(stream, (k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table),
+            lambda s: lib().tllm_kv4_append_f16(k.data_ptr(), v.data_ptr(), ks, vs, cache, batch, s))
 
 
 def kv4_read(k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, stream=None):
@@ -439,8 +436,8 @@ def kv4_read(k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, 
     cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, k.shape[0])
     ks, vs = _rows(k, "k", cache.n_kv_heads), _rows(v, "v", cache.n_kv_heads)
     _want(k.shape == v.shape and k.shape[2] == cache.head_dim, "k and v must be [rows, kv_heads, dim] of the cache")
-    with _on(stream, k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table) as s:
-        check(lib().tllm_kv4_read_f16(_ptr(k), _ptr(v), ks, vs, cache, batch, s))
+    _launch(stream, (k, v, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table),
+            lambda s: lib().tllm_kv4_read_f16(k.data_ptr(), v.data_ptr(), ks, vs, cache, batch, s))
 
 
 def attention_kv4(q, output, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, max_query, max_length, scale=None,
@@ -454,22 +451,27 @@ def attention_kv4(q, output, k_codes, k_scales, v_codes, v_scales, query_starts,
     cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n)
     qs, os_ = _rows(q, "q"), _rows(output, "output")
     _want(output.shape == q.shape and dim == cache.head_dim, "q and output must be [rows, heads, dim] with the cache's dim")
-    with _on(stream, q, output, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table) as s:
-        L = lib()
-        need = L.tllm_attention_kv4_workspace_bytes(cache, batch, heads, max_query, max_length)
-        if need < 0:
-            check(int(need))
-        if workspace is not None:
-            _want(workspace.device == q.device and workspace.is_contiguous(), "the workspace must be contiguous, on the tensors' GPU")
-            have = workspace.numel() * workspace.element_size()
+    if scale is None:
+        scale = dim ** -0.5
+
+    def call(s):
+        L, memory, have = lib(), workspace, 0
+        if memory is not None:
+            _want(memory.is_contiguous(), "the workspace must be contiguous")
+            have = memory.numel() * memory.element_size()
         else:
-            have = need
-            if need:
-                import torch
+            have = L.tllm_attention_kv4_workspace_bytes(cache, batch, heads, max_query, max_length)
+            if have < 0:
+                return have
+            if have:
+                torch = _torch()
                 with torch.cuda.stream(stream):  # (a stream of its own: the allocator hands the memory out in its order)
-                    workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        check(L.tllm_attention_kv4_f16(_ptr(q), _ptr(output), qs, os_, cache, batch, heads, max_query, max_length,
-                                       dim ** -0.5 if scale is None else scale, window, _ptr(workspace), have, s))
+                    memory = torch.empty(have, dtype=torch.uint8, device=q.device)
+        return L.tllm_attention_kv4_f16(q.data_ptr(), output.data_ptr(), qs, os_, cache, batch, heads, max_query, max_length, scale, window,
+                                        None if memory is None else memory.data_ptr(), have, s)
+
+    tensors = (q, output, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table)
+    _launch(stream, tensors if workspace is None else tensors + (workspace,), call)
 
 
 def attention_kv4_workspace_bytes(n_heads, k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n_rows, max_query,
