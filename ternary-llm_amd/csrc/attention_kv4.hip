@@ -21,6 +21,7 @@ typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kEmpty = -1e30f;  // below every score (|q.k| < 2^40, |scale| <= 2^40): no position yet
 constexpr int kHeadroom = 6;      // powers of two that a weight may outgrow its base by before everything is rescaled
@@ -86,7 +87,7 @@ __device__ __forceinline__ int window_begin(const AttentionKv4Args &a, int pos) 
 //
 // Bound: HBM, the cache's 5 bits per value; the work per position has to stay small beside it, above all the work on scores,
 // of which 16 x 16 come out of every matrix instruction however few rows there are. So the row operand repeats its kRows
-// rows (query rows times the heads that share a kv head: 4, 8 or 16), and of kPack = 16 / kRows tiles of 16 positions each
+// rows (query rows times the heads that share a kv head: 4 or 8), and of kPack = 16 / kRows tiles of 16 positions each
 // quad of lanes keeps the results of its own tile: each of the 64 lanes then has ONE position and four rows of its own (lane
 // = (position t, quad)), steps and minima are one coalesced word per lane and group, and softmax runs on four registers. For
 // the values, weights p s go through LDS ([position][group][row], fp16) and come back transposed (ds_read_b64_tr_b16) with
@@ -96,10 +97,14 @@ __device__ __forceinline__ int window_begin(const AttentionKv4Args &a, int pos) 
 // The positions of all sequences are one line of steps, cut into equal pieces, one per wave (each kv head its own line):
 // however ragged the batch, all waves end together. A piece may end inside a sequence and begin inside another; its stretch
 // of a sequence is a segment. A sequence that lies in one piece is stored at once, the segments of others are joined by a
-// second launch. A wave is a workgroup of its own: nothing waits for another wave. Short contexts (at most kAloneSteps steps)
-// take the other form: a workgroup of kAloneWaves waves has a whole row tile, the waves take its steps in turn and meet in
-// LDS, and there is no second launch (517 positions, 8 kv heads: 11 us and 8 + 4 us).
-constexpr int kAloneWaves = 8, kAloneSteps = 16;
+// second launch. A wave is a workgroup of its own: nothing waits for another wave. The other form, for short contexts or
+// many sequences (see plans_of): a workgroup of kAloneWaves waves has a whole row tile, the waves take its steps in turn and
+// meet in LDS, and there is no second launch.
+// Measured (32 query heads, 8 kv heads of 128 dims): 32 sequences of 4096 positions 32 us, a read of their 5 bits 28; the
+// line, 72 000 positions of 32 ragged sequences: 29 us and 5 for the joins, a read 15; 131 072 positions of one sequence with
+// 64 heads: 41 and 6, a read 28. What is left is the vector pipe (some 800 instructions a step of 64 positions, two waves a
+// SIMD for the registers) and, in the line, the chain of loads before a wave's first step and behind its last.
+constexpr int kAloneWaves = 8;
 struct RowPlan {
     int workers;  // waves per kv head
     int tiles;    // row tiles per sequence; row tile t of sequence b is number b * tiles + t of the line
@@ -229,6 +234,28 @@ __device__ __forceinline__ void store_row(const AttentionKv4Args &a, size_t quer
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;  // nothing seen: 0
     const uint2_t packed = {(uint32_t)f2h(o[0] * inv) | (uint32_t)f2h(o[1] * inv) << 16, (uint32_t)f2h(o[2] * inv) | (uint32_t)f2h(o[3] * inv) << 16};
     *(uint2_t *)(a.output + query * a.output_stride + (size_t)head * a.cache.head_dim + d) = packed;
+}
+
+// Joins the sums of a workgroup's waves ([wave][row][dim]) and stores the rows.
+template <int kDim, int kRows, int kWaves>
+__device__ __forceinline__ void join_waves(const AttentionKv4Args &a, const RowTile &tile, int kv, int heads, const float2 (&bases)[kWaves][kRows], const float *sums) {
+    constexpr int kParts = kDim / 4;  // float4s of a row
+    for (int j = threadIdx.x; j < kRows * kParts; j += kWaves * kWave) {
+        const int r = j / kParts, d = j % kParts * 4;
+        if (r >= tile.rows_left) break;
+        float m = kEmpty, all = 0;
+        float4_t o = {};
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) m = fmaxf(m, bases[w][r].x);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            const float keep = __builtin_amdgcn_exp2f(bases[w][r].x - m);
+            all += bases[w][r].y * keep;
+            o += *(const float4_t *)(sums + ((size_t)w * kRows + r) * kDim + d) * keep;
+        }
+        const int at_row = tile.first_row + r;
+        store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d, o, all);
+    }
 }
 
 template <int kDim, int kRows, int kWaves>
@@ -653,23 +680,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
         }
         if constexpr (kAlone) {
             __syncthreads();
-            constexpr int kParts = kDim / 4;  // float4s of a row
-            for (int j = threadIdx.x; j < kRows * kParts; j += kWaves * kWave) {
-                const int r = j / kParts, d = j % kParts * 4;
-                if (r >= tile.rows_left) break;
-                float m = kEmpty, all = 0;
-                float4_t o = {};
-#pragma unroll
-                for (int w = 0; w < kWaves; w++) m = fmaxf(m, join_bases[w][r].x);
-#pragma unroll
-                for (int w = 0; w < kWaves; w++) {
-                    const float keep = __builtin_amdgcn_exp2f(join_bases[w][r].x - m);
-                    all += join_bases[w][r].y * keep;
-                    o += *(const float4_t *)((const float *)lds_all + ((size_t)w * kRows + r) * kDim + d) * keep;
-                }
-                const int at_row = tile.first_row + r;
-                store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d, o, all);
-            }
+            join_waves<kDim, kRows, kWaves>(a, tile, kv, heads, join_bases, (const float *)lds_all);
             return;
         }
         left -= count;
@@ -681,6 +692,279 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
         } while (tile.steps == 0);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- up to 32 rows a tile
+//
+// Bound: the vector pipe, which brings the cache to fp16: a position's 2 kDim values cost some eight instructions a wave, whatever
+// the rows, and a score tile of 32 rows three more. A wave works alone on steps of 32 positions (line or alone, as for few
+// rows), and nothing goes through LDS: a lane brings to fp16 what it is to feed the matrix instructions itself. Products are
+// transposed (k q^T, v^T p^T). For the first a lane has half of one position's dims, in whatever order q's operand repeats; a
+// row's scores then lie in one lane and its partner 32 lanes on, and p is the second product's operand as it lies. Its other
+// operand has dims as rows: a lane has one word's dims of 16 positions, and of the row tiles' order only the stores know. k, v
+// and p are rounded to fp16 (see the next section).
+template <int kDim>
+struct Rows32 {
+    static constexpr int kGroups = kDim / kKvGroup, kWords = kDim / 8;
+    static constexpr int kRows = 32, kStep = 32;
+    static constexpr int kLanesPerWord = 32 / kWords, kNibbles = 8 / kLanesPerWord;  // (kNibbles == kGroups: result tiles)
+    struct Keys {
+        uint4_t k[kGroups / 2];
+        uint32_t scales[kGroups];
+    };
+};
+
+template <int kDim, int kWaves>
+__global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const AttentionKv4Args a, const RowPlan plan) {
+    using R = Rows32<kDim>;
+    constexpr int G = R::kGroups, kRows = R::kRows;
+    constexpr bool kAlone = kWaves > 1;
+    __shared__ __align__(16) float join_sums[kAlone ? kWaves : 1][kAlone ? kRows : 1][kAlone ? kDim : 4];
+    __shared__ float2 join_bases[kAlone ? kWaves : 1][kRows];
+    const Kv4Cache &c = a.cache;
+    const int lane = threadIdx.x % kWave, half = lane >> 5, l32 = lane & 31;
+    const int wave = kAlone ? __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) : 0;
+    const int kv = blockIdx.x, worker = blockIdx.y + blockIdx.z * gridDim.y;
+    if (worker >= plan.workers) return;
+    const int heads = a.n_heads / c.n_kv_heads, numbers = a.batch.batch * plan.tiles;
+    int number = worker, offset = 0, left = INT32_MAX;
+    RowTile tile;
+    if constexpr (kAlone) {
+        tile = RowTile(a, plan, number, kRows, R::kStep);
+        if (tile.rows_left <= 0) return;
+    } else {
+        const bool scribe = kv == 0 && worker == 0;
+        const Segments segments(a, plan, kRows);
+        if (!find_piece(a, plan, worker, kRows, R::kStep, scribe, scribe ? segments.parts : nullptr, &number, &offset, &left, &tile)) return;
+    }
+    const int limit = position_limit(a);
+    const size_t code_words = kv4_code_words(1 << c.page_shift, kDim), scale_words = kv4_scale_words(1 << c.page_shift, kDim);
+    const int v_word = l32 % R::kWords, v_part = l32 / R::kWords;
+    // this lane's bytes in 16 positions of a page
+    const uint32_t key_offset = (uint32_t)((l32 & 15) * R::kWords + half * 2 * G) * 4, key_scale_offset = (uint32_t)(l32 & 15) * 4;
+    const uint32_t value_offset = (uint32_t)(half * R::kWords + v_word) * 16, value_scale_offset = (((uint32_t)(v_word / 4) << c.page_shift) + 4 * half) * 4;
+    const float to_log2 = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * (2.0f * 1.44269504088896f);
+    // half of a code in fp16: 512 + c / 2 (32 + c / 2 from bits 4-7) less the rest
+    uint32_t even_bits = 0x60006000u, odd_bits = 0x50005000u;  // (in registers: two constants make two instructions)
+    asm("" : "+v"(even_bits), "+v"(odd_bits));
+    auto value2 = [&](uint32_t field, bool odd, half2_t s, half2_t m) {
+        const half2_t code = __builtin_bit_cast(half2_t, odd ? (field & kOddCodes) | odd_bits : (field & kEvenCodes) | even_bits) - (odd ? half2_t{32, 32} : half2_t{512, 512});
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, s, m));
+    };
+
+    while (true) {
+        const int count = min(tile.steps - offset, left);
+        const bool entire = kAlone || (offset == 0 && count == tile.steps);
+        const int *table = a.batch.table + (size_t)(plan.tiles == 1 ? number : number / plan.tiles) * a.batch.width;
+        int step = tile.first_step + offset + wave;
+        const int end = tile.first_step + offset + count;
+
+        // 64 entries of the page table at a time, one per lane
+        int held_from = (tile.first_step + offset) * R::kStep >> c.page_shift, held = table[min(held_from + lane, a.batch.width - 1)];
+        uint32_t block[2], slot[2], there = 0;  // of each 16 positions: page * n_kv_heads + head, first slot; bit i: they have a page
+        auto find = [&] {
+            const int at = step * R::kStep;
+            if ((at + 16) >> c.page_shift >= held_from + kWave) {
+                held_from = at >> c.page_shift;
+                held = table[min(held_from + lane, a.batch.width - 1)];
+            }
+            there = 0;
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                const int index = (at + 16 * i) >> c.page_shift, page = __builtin_amdgcn_readlane(held, index - held_from);
+                const bool real = index < a.batch.width && page >= 0 && page < c.n_pages;
+                there |= (uint32_t)real << i;
+                block[i] = (real ? page : 0) * c.n_kv_heads + kv;
+                slot[i] = (at + 16 * i) & ((1 << c.page_shift) - 1);
+            }
+        };
+        const auto bytes = [](const void *at, size_t words) { return (const unsigned char *)at + words * 4; };
+        auto load_keys = [&](typename R::Keys &x) {
+            const bool second = l32 >= 16;
+            const unsigned char *codes[2], *scales[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                codes[i] = bytes(c.k_codes, block[i] * code_words + (size_t)slot[i] * R::kWords);
+                scales[i] = bytes(c.k_scales, block[i] * scale_words + slot[i]);
+            }
+            const unsigned char *from = (second ? codes[1] : codes[0]) + key_offset, *scale = (second ? scales[1] : scales[0]) + key_scale_offset;
+#pragma unroll
+            for (int i = 0; i < G / 2; i++) x.k[i] = ((const uint4_t *)from)[i];
+#pragma unroll
+            for (int g = 0; g < G; g++) x.scales[g] = *(const uint32_t *)(scale + ((size_t)g << (c.page_shift + 2)));
+        };
+
+        // this lane's row, and its operand: depth (word pair, odd or even, quad) of a key's order
+        const int at_row = tile.first_row + l32;
+        const bool real = l32 < tile.rows_left;
+        const size_t query = (size_t)(tile.row0 + (real ? at_row / heads : 0));
+        const int head = kv * heads + (real ? at_row % heads : 0), pos = real ? tile.pos0 + at_row / heads : -1;
+        half8_t q[2 * G];
+#pragma unroll
+        for (int k = 0; k < 2 * G; k++) {
+            q[k] = real ? *(const half8_t *)(a.q + query * a.q_stride + (size_t)head * kDim + (k >> 1) * 32 + (2 * half + (k & 1)) * 8) : half8_t{};
+            if (a.scale < 0) q[k] = -q[k];
+            if (a.scale == 0) q[k] = half8_t{};
+        }
+        typename R::Keys now;
+        if (step < end) {
+            find();
+            load_keys(now);
+        }
+        float16_t acc[G] = {};
+        float sum = 0, base = kEmpty;
+        while (step < end) {
+            // this step's values, which the work on the scores covers, then the next step's keys
+            uint4_t v[4], v_scales[4];  // [8 positions]: four of them, of this lane's word; their steps and minima
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                v[i] = *(const uint4_t *)(bytes(c.v_codes, block[i >> 1] * code_words + (size_t)slot[i >> 1] * R::kWords + (i & 1) * 8 * R::kWords) + value_offset);
+                v_scales[i] = *(const uint4_t *)(bytes(c.v_scales, block[i >> 1] * scale_words + slot[i >> 1] + (i & 1) * 8) + value_scale_offset);
+            }
+            const uint32_t pages = there;
+            const int first = step * R::kStep;
+            typename R::Keys next;
+            step += kWaves;
+            if (step < end) {
+                find();
+                load_keys(next);
+            }
+            const bool whole = pages == 3 && first + R::kStep - 1 <= tile.pos_low && first + R::kStep <= limit && (a.window == 0 || first > tile.pos_high - a.window);
+            float16_t x = {};
+#pragma unroll
+            for (int quad = 0; quad < 2; quad++)
+#pragma unroll
+                for (int pair = 0; pair < G / 2; pair++) {
+                    const int word = quad * G + 2 * pair;
+                    const uint32_t w0 = now.k[word >> 2][word & 3], w1 = now.k[word >> 2][(word & 3) + 1];
+#pragma unroll
+                    for (int odd = 0; odd < 2; odd++) {
+                        const half2_t both = __builtin_bit_cast(half2_t, now.scales[2 * pair + odd]) * half2_t{1, 0.5f};
+                        const half2_t s = {both[0], both[0]}, m = {both[1], both[1]};
+                        const uint4_t key = {value2(w0, odd, s, m), value2(w0 >> 8, odd, s, m), value2(w1, odd, s, m), value2(w1 >> 8, odd, s, m)};
+                        x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, key), q[(2 * pair + odd) * 2 + quad], x, 0, 0, 0);
+                    }
+                }
+            if (!whole) {
+                asm volatile("");  // (a branch: not worked out and chosen from in every step)
+#pragma unroll
+                for (int j = 0; j < 16; j++) {
+                    const int t = first + 8 * (j >> 2) + 4 * half + (j & 3);
+                    const bool sees = t <= pos && t < limit && (a.window == 0 || t > pos - a.window) && (pages >> (j >> 3) & 1);
+                    x[j] = sees ? x[j] : -INFINITY;
+                }
+            }
+            float most = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 16; j++) most = fmaxf(most, x[j]);
+            most = fmaxf(most, __shfl_xor(most, 32, kWave)) * to_log2;
+            if (__ballot(most - base > 14.0f)) {
+                const float to = fmaxf(base, most - 6.0f), keep = __builtin_amdgcn_exp2f(base - to);
+                base = to;
+                sum *= keep;
+#pragma unroll
+                for (int g = 0; g < G; g++) acc[g] *= keep;
+            }
+            half8_t weights[2];
+#pragma unroll
+            for (int j = 0; j < 16; j++) weights[j >> 3][j & 7] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(x[j], to_log2, -base));
+#pragma unroll
+            for (int j = 0; j < 16; j += 2)  // (of the rounded weights, which is what the values are multiplied with)
+                sum = __builtin_amdgcn_fdot2(half2_t{weights[j >> 3][j & 7], weights[j >> 3][(j & 7) + 1]}, half2_t{1, 1}, sum, false);
+
+            // what no row sees may be anything: its values are zeros (its weights are). So are groups that are not finite, and
+            // the rows that see them get a NaN
+            uint32_t odd_one = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) odd_one |= (v_scales[i][j] & 0x7C007C00u) + 0x04000400u;  // bits 15 and 31: an exponent is all ones
+            if (!whole || __ballot(odd_one & 0x80008000u)) {
+                asm volatile("");
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int t = first + 8 * i + j;  // (of the lower half of the lanes)
+                        const int own = t + 4 * half;
+                        const bool seen = (pages >> (i >> 1) & 1) && own <= tile.pos_high && own < limit && (a.window == 0 || own > tile.pos_low - a.window);
+                        const bool bad = seen && ((v_scales[i][j] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                        v_scales[i][j] = seen && !bad ? v_scales[i][j] : 0;
+                        const unsigned long long all_bad = __ballot(bad);
+                        if (all_bad) {
+                            for (int h = 0; h < 2; h++) {
+                                const int its = t + 4 * h;
+                                const bool sees = its <= pos && (a.window == 0 || its > pos - a.window);
+#pragma unroll
+                                for (int e = 0; e < 16; e++) {
+                                    const int group = (2 * (e >> 2) + half) % G;  // of this lane's results e
+                                    if (sees && (all_bad >> (32 * h + 4 * group) & 1)) {
+#pragma unroll
+                                        for (int g = 0; g < G; g++) acc[g][e] = NAN;
+                                    }
+                                }
+                            }
+                        }
+                    }
+            }
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                uint4_t values[R::kNibbles];
+#pragma unroll
+                for (int b = 0; b < 2; b++) {
+                    const uint4_t words = v[2 * k + b], pairs = v_scales[2 * k + b];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const half2_t s = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(pairs[2 * j + 1], pairs[2 * j], 0x05040100u));
+                        const half2_t m = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(pairs[2 * j + 1], pairs[2 * j], 0x07060302u)) * half2_t{0.5f, 0.5f};
+#pragma unroll
+                        for (int byte = 0; byte < R::kNibbles / 2; byte++) {
+                            // this lane's byte `byte` of two positions' words, one per half
+                            const uint32_t which = (uint32_t)(v_part * (R::kNibbles / 2) + byte), select = which * 0x00010001u + 0x0C040C00u;
+                            const uint32_t field = __builtin_amdgcn_perm(words[2 * j + 1], words[2 * j], select);
+                            values[2 * byte][2 * b + j] = value2(field, false, s, m);
+                            values[2 * byte + 1][2 * b + j] = value2(field, true, s, m);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < R::kNibbles; n++) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, values[n]), weights[k], acc[n], 0, 0, 0);
+            }
+            now = next;
+        }
+
+        sum += __shfl_xor(sum, 32, kWave);
+        if (kAlone && half == 0) join_bases[wave][l32] = make_float2(base, sum);
+        const Segments segments(a, plan, kRows);
+        const size_t place = ((size_t)kv * segments.per_head + worker + number) * kRows + l32;
+        if (!entire && real && half == 0) *(float2 *)(segments.bases + place * 2) = make_float2(base, sum);
+        const float inv = sum == 0.0f ? 0.0f : 2.0f / sum;  // (half of v was taken); nothing seen: 0
+        if (kAlone || real) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const int at = 8 * (e >> 2) + 4 * half + (e & 3), d = at % R::kWords * 8 + at / R::kWords * R::kNibbles;  // first of kNibbles dims
+                float *to = kAlone ? &join_sums[wave][kAlone ? l32 : 0][kAlone ? d : 0] : segments.sums + place * kDim + d;
+                uint16_t *out = a.output + query * a.output_stride + (size_t)head * kDim + d;
+#pragma unroll
+                for (int n = 0; n < R::kNibbles; n += 2) {
+                    if (!kAlone && entire) *(uint32_t *)(out + n) = (uint32_t)f2h(acc[n][e] * inv) | (uint32_t)f2h(acc[n + 1][e] * inv) << 16;
+                    else *(float2 *)(to + n) = make_float2(acc[n][e] * 2.0f, acc[n + 1][e] * 2.0f);
+                }
+            }
+        }
+        if constexpr (kAlone) {
+            __syncthreads();
+            join_waves<kDim, kRows, kWaves>(a, tile, kv, heads, join_bases, (const float *)join_sums);
+            return;
+        }
+        left -= count;
+        if (left <= 0) return;
+        offset = 0;
+        do {
+            if (++number >= numbers) return;
+            tile = RowTile(a, plan, number, kRows, R::kStep);
+        } while (tile.steps == 0);
     }
 }
 
@@ -772,8 +1056,6 @@ struct Prompt {
     static constexpr int kKeyTile = kTile * kKeyBytes, kStage = kKeyTile + kDim * kValueBytes;
     static constexpr int kChunk = 64, kSub = kChunk / 32, kDepths = kDim / 16;  // positions that a wave has scores of at once
 };
-typedef float float16_t __attribute__((ext_vector_type(16)));
-
 template <int kDim, int kWaves>
 __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(const AttentionKv4Args a, const RowPlan plan, size_t segments_at) {
     using P = Prompt<kDim, kWaves>;
@@ -1070,10 +1352,14 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
 
 // ------------------------------------------------------------------------------------------------- launches
 
-constexpr int kFewRows = 64;  // (query rows times heads of a kv head) that go the way of few rows
+// Rows (query rows times heads of a kv head) up to which a sequence goes the way of few rows. 16 sequences of 8192 positions,
+// 64 rows each: 109 us, 138 as a prompt; 128 rows: 181 and 140. (One sequence of 8192 positions, 64 rows: 35 and 20.)
+constexpr int kFewRows = 64;
 
-int decode_rows(long long rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 16; }
-int decode_step(int rows) { return rows == 4 ? 64 : 32; }
+// Rows of a tile: 4 and 8 take bare codes, 32 values brought to fp16. 8 rows, 131 072 positions: 47 us with 8, 56 with 32; 4
+// rows, 72 000 positions: 34 with 4, 42 with 32. (Bare codes with 16 rows a tile took as long as 32 rows take now: 60 us for
+// 16 rows of 16 sequences of 8192, and 99 for 32.)
+int decode_rows(long long rows) { return rows <= 4 ? 4 : rows <= 8 ? 8 : 32; }
 
 // What a call launches: for sequences of few rows, for sequences of many, or both.
 struct Plans {
@@ -1084,11 +1370,9 @@ struct Plans {
     size_t few_bytes, many_bytes;
 };
 
-// Steps that a row tile may have, as far as the host knows.
-long long most_steps(const AttentionKv4Args &a, int step) {
-    long long reach = a.max_length;
-    if (a.window > 0 && (long long)a.window + a.max_query < reach) reach = (long long)a.window + a.max_query;
-    return (reach + step - 1) / step + 1;
+// Positions that a row tile may see, as far as the host knows.
+long long reach(const AttentionKv4Args &a) {
+    return a.window > 0 ? std::min((long long)a.window + a.max_query, (long long)a.max_length) : a.max_length;
 }
 
 constexpr int kPromptWaves = 8;
@@ -1104,8 +1388,16 @@ Plans plans_of(const AttentionKv4Args &a) {
     if (p.few) {
         const long long most = std::min<long long>(rows, kFewRows);
         p.few_rows = decode_rows(most);
-        p.few_plan = RowPlan{0, (int)((most + p.few_rows - 1) / p.few_rows), 1, 0, 0, p.many ? kFewRows + 1 : INT32_MAX};
-        p.few_plan.alone = most_steps(a, decode_step(p.few_rows)) <= kAloneSteps;
+        // (32 rows' sums are 16 KB a segment: fewer, of four steps at least. One sequence of 8192 positions and 16 rows: 18 us,
+        // with one step at least 24, with eight 23)
+        p.few_plan = RowPlan{0, (int)((most + p.few_rows - 1) / p.few_rows), p.few_rows == 32 ? 4 : 1, 0, 0, p.many ? kFewRows + 1 : INT32_MAX};
+        // A row tile a workgroup takes the time of its positions on one CU, 8 us and some 5 per 1024; the line takes 11 us and
+        // what all positions cost on all CUs. 4 rows, 1 sequence: 512 positions 10 us alone and 11 in line, 1024 12 and 12,
+        // 2048 18 and 12; 8 sequences (64 workgroups): 1024 13 and 14, 2048 18 and 17, 4096 30 and 22; 32 (256): 4096 32 and
+        // 39. Only a bound of the lengths is known here: a single long sequence among many short ones costs more alone (8192
+        // among 200 to 8192: 51 us, in line 34), so that 4096 positions are the most.
+        const long long groups = (long long)a.batch.batch * p.few_plan.tiles * kv;
+        p.few_plan.alone = reach(a) <= std::min(512 + 16 * groups, 4096ll);
         // two waves a SIMD
         p.few_plan.workers = p.few_plan.alone ? a.batch.batch * p.few_plan.tiles : (8 * cus + kv - 1) / kv;
         p.few_bytes = p.few_plan.alone ? 0 : (Segments::bytes(a, p.few_plan, p.few_rows) + 15) / 16 * 16;
@@ -1116,7 +1408,7 @@ Plans plans_of(const AttentionKv4Args &a) {
         p.many_plan = RowPlan{0, (int)((rows + tile_rows - 1) / tile_rows), 1, 0, p.few ? kFewRows + 1 : 0, INT32_MAX};
         const long long tiles = (long long)a.batch.batch * p.many_plan.tiles;
         const int slots = 8 / p.many_waves * cus;  // two waves a SIMD
-        p.many_plan.alone = tiles * kv >= slots || most_steps(a, step) <= 4;
+        p.many_plan.alone = tiles * kv >= slots || (reach(a) + step - 1) / step <= 3;
         p.many_plan.workers = p.many_plan.alone ? (int)tiles : (slots + kv - 1) / kv;
         p.many_plan.least = 2;
         p.many_bytes = p.many_plan.alone ? 0 : Segments::bytes(a, p.many_plan, tile_rows);
@@ -1138,6 +1430,17 @@ hipError_t launch_join(const AttentionKv4Args &a, const RowPlan &plan, size_t se
     else
         attention_join_kernel<kDim, kRows, kStep, kDim / 4><<<dim3(tiles, kv, kRows / 4), kJoinThreads, lds, s>>>(a, plan, segments_at);
     return hipGetLastError();
+}
+
+template <int kDim>
+hipError_t launch_rows32(const AttentionKv4Args &a, const RowPlan &plan, hipStream_t s) {
+    if (plan.alone) {
+        attention_rows_kernel<kDim, kAloneWaves><<<worker_grid(a, plan), kAloneWaves * kWave, 0, s>>>(a, plan);
+        return hipGetLastError();
+    }
+    attention_rows_kernel<kDim, 1><<<worker_grid(a, plan), kWave, 0, s>>>(a, plan);
+    if (hipError_t e = hipGetLastError()) return e;
+    return launch_join<kDim, 32, Rows32<kDim>::kStep>(a, plan, 0, s);
 }
 
 template <int kDim, int kRows>
@@ -1168,7 +1471,7 @@ hipError_t launch(const AttentionKv4Args &a, hipStream_t s) {
     switch (p.few_rows) {
         case 4: return launch_few<kDim, 4>(a, p.few_plan, s);
         case 8: return launch_few<kDim, 8>(a, p.few_plan, s);
-        default: return launch_few<kDim, 16>(a, p.few_plan, s);
+        default: return launch_rows32<kDim>(a, p.few_plan, s);
     }
 }
 
