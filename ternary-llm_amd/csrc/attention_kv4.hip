@@ -117,7 +117,8 @@ template <int kDim, int kRows>
 struct Decode {
     static constexpr int kGroups = kDim / kKvGroup, kWords = kDim / 8;
     static constexpr int kPack = 16 / kRows;
-    static constexpr int kTiles = kRows == 4 ? 4 : 2, kStep = 16 * kTiles, kPasses = kTiles / kPack;
+    static constexpr int kTiles = kRows == 4 ? 4 : 2, kStep = 16 * kTiles;
+    static_assert(kTiles == kPack, "a position per lane");
     static constexpr int kColumns = kGroups * kRows < 16 ? 16 : kGroups * kRows;  // of the weights: (group, row)
     static constexpr int kSets = kColumns / 16, kSetGroups = kGroups / kSets;
     static constexpr int kSetWords = 4 * kSetGroups, kLanesPerWord = 16 / kSetWords, kNibbles = 8 / kLanesPerWord;
@@ -131,7 +132,7 @@ struct Decode {
     };
     struct Keys {
         KeyWords k[kTiles];
-        uint32_t km[kPasses][kGroups], vm[kPasses][kGroups];  // step | minimum << 16 of this lane's position, keys and values
+        uint32_t km[kGroups], vm[kGroups];  // step | minimum << 16 of this lane's position, keys and values
     };
     struct Values {
         uint4_t v[kTiles][kSets];
@@ -334,25 +335,20 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
             if (one_page) {
                 const size_t word = at.block[0] * scale_words + at.slot[0];
 #pragma unroll
-                for (int g = 0; g < G; g++)
-#pragma unroll
-                    for (int p = 0; p < D::kPasses; p++) {
-                        x.km[p][g] = *(const uint32_t *)(bytes(c.k_scales, word + ((size_t)g << c.page_shift)) + scale_offset + p * D::kPack * 64);
-                        x.vm[p][g] = *(const uint32_t *)(bytes(c.v_scales, word + ((size_t)g << c.page_shift)) + scale_offset + p * D::kPack * 64);
-                    }
+                for (int g = 0; g < G; g++) {
+                    x.km[g] = *(const uint32_t *)(bytes(c.k_scales, word + ((size_t)g << c.page_shift)) + scale_offset);
+                    x.vm[g] = *(const uint32_t *)(bytes(c.v_scales, word + ((size_t)g << c.page_shift)) + scale_offset);
+                }
             } else {
+                uint32_t b = at.block[0], sl = at.slot[0];
 #pragma unroll
-                for (int p = 0; p < D::kPasses; p++) {
-                    uint32_t b = at.block[p * D::kPack], sl = at.slot[p * D::kPack];
+                for (int u = 1; u < D::kPack; u++)
+                    if (pack == u) b = at.block[u], sl = at.slot[u];
+                const size_t word = b * scale_words + sl + t16;
 #pragma unroll
-                    for (int u = 1; u < D::kPack; u++)
-                        if (pack == u) b = at.block[p * D::kPack + u], sl = at.slot[p * D::kPack + u];
-                    const size_t word = b * scale_words + sl + t16;
-#pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        x.km[p][g] = c.k_scales[word + ((size_t)g << c.page_shift)];
-                        x.vm[p][g] = c.v_scales[word + ((size_t)g << c.page_shift)];
-                    }
+                for (int g = 0; g < G; g++) {
+                    x.km[g] = c.k_scales[word + ((size_t)g << c.page_shift)];
+                    x.vm[g] = c.v_scales[word + ((size_t)g << c.page_shift)];
                 }
             }
         };
@@ -421,81 +417,78 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
             // whole: every row sees all of the step's positions
             const bool whole = pages == (1u << D::kTiles) - 1 && first + D::kStep - 1 <= tile.pos_low && first + D::kStep <= limit &&
                                (a.window == 0 || first > tile.pos_high - a.window);
-            float raw[D::kPasses][4], most = -INFINITY;
-            uint32_t largest = 0, sees = ~0u;  // sees: bit 4 p + r
+            float raw[4], most = -INFINITY;
+            uint32_t largest = 0, sees = ~0u;  // sees: a bit per row r
+            float4_t d[G];
 #pragma unroll
-            for (int p = 0; p < D::kPasses; p++) {
-                float4_t d[G];
+            for (int pair = 0; pair < G / 2; pair++)
 #pragma unroll
-                for (int pair = 0; pair < G / 2; pair++)
-#pragma unroll
-                    for (int u = 0; u < D::kPack; u++) {
-                        const uint32_t w0 = now.k[p * D::kPack + u][2 * pair], w1 = now.k[p * D::kPack + u][2 * pair + 1];
-                        const uint4_t even = {w0 & kEvenCodes, w0 >> 8 & kEvenCodes, w1 & kEvenCodes, w1 >> 8 & kEvenCodes};
-                        const uint4_t odd = {w0 & kOddCodes, w0 >> 8 & kOddCodes, w1 & kOddCodes, w1 >> 8 & kOddCodes};
-                        const float4_t d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair], __builtin_bit_cast(half8_t, even), float4_t{}, 0, 0, 0);
-                        const float4_t d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair + 1], __builtin_bit_cast(half8_t, odd), float4_t{}, 0, 0, 0);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            d[2 * pair][r] = u == 0 || pack == u ? d0[r] : d[2 * pair][r];
-                            d[2 * pair + 1][r] = u == 0 || pack == u ? d1[r] : d[2 * pair + 1][r];
-                        }
-                        if (u & 1) __builtin_amdgcn_sched_barrier(0);
-                    }
-                bool unsound = false;
-                if (!whole) {
-                    asm volatile("");  // (a branch: not worked out and chosen from in every step)
-                    const int t = first + 16 * (p * D::kPack + pack) + t16;
-                    const bool there = (pages >> (p * D::kPack + pack) & 1) && t < limit;
+                for (int u = 0; u < D::kPack; u++) {
+                    const uint32_t w0 = now.k[u][2 * pair], w1 = now.k[u][2 * pair + 1];
+                    const uint4_t even = {w0 & kEvenCodes, w0 >> 8 & kEvenCodes, w1 & kEvenCodes, w1 >> 8 & kEvenCodes};
+                    const uint4_t odd = {w0 & kOddCodes, w0 >> 8 & kOddCodes, w1 & kOddCodes, w1 >> 8 & kOddCodes};
+                    const float4_t d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair], __builtin_bit_cast(half8_t, even), float4_t{}, 0, 0, 0);
+                    const float4_t d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair + 1], __builtin_bit_cast(half8_t, odd), float4_t{}, 0, 0, 0);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
-                        const int row = 4 * row_quad + r, pos = tile.pos0 + (tile.first_row + row) / heads;
-                        const bool one = there && row < tile.rows_left && t <= pos && (a.window == 0 || t > pos - a.window);
-                        sees &= ~((uint32_t)!one << (4 * p + r));
+                        d[2 * pair][r] = u == 0 || pack == u ? d0[r] : d[2 * pair][r];
+                        d[2 * pair + 1][r] = u == 0 || pack == u ? d1[r] : d[2 * pair + 1][r];
                     }
-                    // What no row sees may be anything, and must reach neither the powers below nor, in the product of the
-                    // minima, the other tiles' positions. Nor must what is not finite and only some rows see reach the others:
-                    // a key's rows get their NaN in the scores below, a value's in the sum of its group's minima.
-                    const bool any = there && t <= tile.pos_high && (a.window == 0 || t > tile.pos_low - a.window);
-#pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        unsound |= any && (now.km[p][g] & 0x7C000000u) == 0x7C000000u;
-                        const bool wrong = any && ((now.vm[p][g] & 0x7C000000u) == 0x7C000000u || (now.vm[p][g] & 0x7C00u) == 0x7C00u);
-                        now.vm[p][g] = any && !wrong ? now.vm[p][g] : 0;
-#pragma unroll
-                        for (int r = 0; r < 4; r++) acc_min[g][r] = wrong && (sees >> (4 * p + r) & 1) ? NAN : acc_min[g][r];
-                    }
-#pragma unroll
-                    for (int g = 0; g < G; g++) now.km[p][g] = any && !unsound ? now.km[p][g] : 0;
+                    if (u & 1) __builtin_amdgcn_sched_barrier(0);
                 }
-                uint4_t minima;
-#pragma unroll
-                for (int j = 0; j < 4; j++)  // (G is 2: the last four depths have zero rows, and zeros here)
-                    minima[j] = G == 4 || j < 2 ? __builtin_amdgcn_perm(now.km[p][2 * j % G + 1], now.km[p][2 * j % G], 0x07060302u) : 0;
-                const float4_t low = __builtin_amdgcn_mfma_f32_16x16x32_f16(q_sums, __builtin_bit_cast(half8_t, minima), float4_t{}, 0, 0, 0);
+            bool unsound = false;
+            if (!whole) {
+                asm volatile("");  // (a branch: not worked out and chosen from in every step)
+                const int t = first + 16 * pack + t16;
+                const bool there = (pages >> pack & 1) && t < limit;
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    float even = 0, odd = 0;
-#pragma unroll
-                    for (int g = 0; g < G; g += 2) {
-                        even = __builtin_fmaf(low_half(now.km[p][g]), d[g][r], even);
-                        odd = __builtin_fmaf(low_half(now.km[p][g + 1]), d[g + 1][r], odd);
-                    }
-                    raw[p][r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low[r] * (32.0f * c_low)));
+                    const int row = 4 * row_quad + r, pos = tile.pos0 + (tile.first_row + row) / heads;
+                    const bool one = there && row < tile.rows_left && t <= pos && (a.window == 0 || t > pos - a.window);
+                    sees &= ~((uint32_t)!one << r);
                 }
-                if (!whole) {
-                    asm volatile("");
+                // What no row sees may be anything, and must reach neither the powers below nor, in the product of the
+                // minima, the other tiles' positions. Nor must what is not finite and only some rows see reach the others:
+                // a key's rows get their NaN in the scores below, a value's in the sum of its group's minima.
+                const bool any = there && t <= tile.pos_high && (a.window == 0 || t > tile.pos_low - a.window);
 #pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        raw[p][r] = unsound ? NAN : raw[p][r];
-                        raw[p][r] = sees >> (4 * p + r) & 1 ? raw[p][r] : -INFINITY;
-                    }
+                for (int g = 0; g < G; g++) {
+                    unsound |= any && (now.km[g] & 0x7C000000u) == 0x7C000000u;
+                    const bool wrong = any && ((now.vm[g] & 0x7C000000u) == 0x7C000000u || (now.vm[g] & 0x7C00u) == 0x7C00u);
+                    now.vm[g] = any && !wrong ? now.vm[g] : 0;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc_min[g][r] = wrong && (sees >> r & 1) ? NAN : acc_min[g][r];
                 }
 #pragma unroll
-                for (int r = 0; r < 4; r++) most = fmaxf(most, raw[p][r] - base[r]);
-#pragma unroll
-                for (int g = 0; g < G; g++) largest = max(largest, now.vm[p][g] & 0xFFFFu);
+                for (int g = 0; g < G; g++) now.km[g] = any && !unsound ? now.km[g] : 0;
             }
+            uint4_t minima;
+#pragma unroll
+            for (int j = 0; j < 4; j++)  // (G is 2: the last four depths have zero rows, and zeros here)
+                minima[j] = G == 4 || j < 2 ? __builtin_amdgcn_perm(now.km[2 * j % G + 1], now.km[2 * j % G], 0x07060302u) : 0;
+            const float4_t low = __builtin_amdgcn_mfma_f32_16x16x32_f16(q_sums, __builtin_bit_cast(half8_t, minima), float4_t{}, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                float even = 0, odd = 0;
+#pragma unroll
+                for (int g = 0; g < G; g += 2) {
+                    even = __builtin_fmaf(low_half(now.km[g]), d[g][r], even);
+                    odd = __builtin_fmaf(low_half(now.km[g + 1]), d[g + 1][r], odd);
+                }
+                raw[r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low[r] * (32.0f * c_low)));
+            }
+            if (!whole) {
+                asm volatile("");
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    raw[r] = unsound ? NAN : raw[r];
+                    raw[r] = sees >> r & 1 ? raw[r] : -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) most = fmaxf(most, raw[r] - base[r]);
+#pragma unroll
+            for (int g = 0; g < G; g++) largest = max(largest, now.vm[g] & 0xFFFFu);
             const bool grown = most > (float)(kHeadroom + kTopPower - power) || largest > power_bits;
             if (__ballot(grown)) {
                 // rare after the first steps: new bases (a base is the row's largest score so far, moved by the powers)
@@ -513,10 +506,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
                 float keep[4];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    float m = raw[0][r];
-#pragma unroll
-                    for (int p = 1; p < D::kPasses; p++) m = fmaxf(m, raw[p][r]);
-                    m = quad_max(m);
+                    float m = quad_max(raw[r]);
 #pragma unroll
                     for (int off = 4 * kRows; off < kWave; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
                     const float to = fmaxf(base[r] - moved, m) + (float)(power - kTopPower);
@@ -538,35 +528,32 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
 #pragma unroll
                     for (int i = 0; i < D::kNibbles; i++) acc[e][i] *= column;
             }
+            float w[4];
 #pragma unroll
-            for (int p = 0; p < D::kPasses; p++) {
-                float w[4];
+            for (int r = 0; r < 4; r++) {
+                w[r] = __builtin_amdgcn_exp2f(raw[r] - base[r]);
+                sum[r] += w[r];
+            }
+            unsigned char *to = lds + (16 * pack + t16) * D::kRowBytes + row_quad * 8;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const float size = low_half(now.vm[g]) * sign, low = __builtin_fmaf(low_half(now.vm[g]), flipped, high_half(now.vm[g]));
+                float ws[4];
+                uint32_t hi[2], lo[2];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    w[r] = __builtin_amdgcn_exp2f(raw[p][r] - base[r]);
-                    sum[r] += w[r];
+                    ws[r] = w[r] * size;
+                    acc_min[g][r] = __builtin_fmaf(w[r], low, acc_min[g][r]);
                 }
-                unsigned char *to = lds + (16 * (p * D::kPack + pack) + t16) * D::kRowBytes + row_quad * 8;
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    const float size = low_half(now.vm[p][g]) * sign, low = __builtin_fmaf(low_half(now.vm[p][g]), flipped, high_half(now.vm[p][g]));
-                    float ws[4];
-                    uint32_t hi[2], lo[2];
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        ws[r] = w[r] * size;
-                        acc_min[g][r] = __builtin_fmaf(w[r], low, acc_min[g][r]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const half2_t h = {(_Float16)ws[2 * j], (_Float16)ws[2 * j + 1]};
-                        const half2_t l = {(_Float16)__builtin_fmaf((float)h[0], minus_one, ws[2 * j]), (_Float16)__builtin_fmaf((float)h[1], minus_one, ws[2 * j + 1])};
-                        hi[j] = __builtin_bit_cast(uint32_t, h);
-                        lo[j] = __builtin_bit_cast(uint32_t, l);
-                    }
-                    *(uint2_t *)(to + g * kRows * 2) = uint2_t{hi[0], hi[1]};
-                    *(uint2_t *)(to + D::kColumns * 2 + g * kRows * 2) = uint2_t{lo[0], lo[1]};
+                for (int j = 0; j < 2; j++) {
+                    const half2_t h = {(_Float16)ws[2 * j], (_Float16)ws[2 * j + 1]};
+                    const half2_t l = {(_Float16)__builtin_fmaf((float)h[0], minus_one, ws[2 * j]), (_Float16)__builtin_fmaf((float)h[1], minus_one, ws[2 * j + 1])};
+                    hi[j] = __builtin_bit_cast(uint32_t, h);
+                    lo[j] = __builtin_bit_cast(uint32_t, l);
                 }
+                *(uint2_t *)(to + g * kRows * 2) = uint2_t{hi[0], hi[1]};
+                *(uint2_t *)(to + D::kColumns * 2 + g * kRows * 2) = uint2_t{lo[0], lo[1]};
             }
             // (the lanes read each other's weights: the wave's LDS accesses run in order, the compiler has to keep it)
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
