@@ -368,11 +368,13 @@ int tllm_kv4_read_f16(uint16_t *k, uint16_t *v, int64_t k_stride, int64_t v_stri
  * prompts are the same call; sequences of a batch may differ in it.
  * max_query and max_length are upper bounds the host knows: rows of a sequence from max_query on are left as they were, positions from
  * max_length on are not seen. They size the launch, so tight ones are faster; for a captured graph take the largest of
- * its replays. Scores, softmax statistics and sums are fp32, products fp16 x fp16 with exact fp32 accumulation; no atomics:
- * the same call gives the same bits.
+ * its replays. The same call gives the same bits.
+ * Scores, softmax statistics and sums are fp32. Up to 8 rows of a kv head (a sequence's rows times n_heads / n_kv_heads)
+ * multiply q with the codes themselves and take weights in two fp16 pieces: next to the result's own rounding nothing is
+ * rounded to fewer than 22 bits. From 9 rows on k, v and p are rounded to fp16 (2^-11 each) before their products.
  * workspace: tllm_attention_kv4_workspace_bytes() bytes of device memory, 16-byte aligned (NULL when that is 0), used during
  * the call only, contents do not matter; calls that may overlap in time need one each. TLLM_ERR_SCRATCH_TOO_SMALL if less.
- * Few rows over long contexts are shared out along the positions and joined through it. It depends on the
+ * Few row tiles over long contexts are shared out along the positions and joined through it. It depends on the
  * sizes and on the current device, not on the arrays' contents. Negative: a TLLM_ERR_* code.
  * Limits: n_heads a multiple of n_kv_heads, <= 4096; 1 <= max_query, max_length; n_heads * max_query <= 2^27; |scale| <= 2^40.
  * The reference's counterpart for an fp16 cache is kernels/attention.cu:30-333.

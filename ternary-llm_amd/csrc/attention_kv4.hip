@@ -237,8 +237,8 @@ __device__ __forceinline__ void store_row(const AttentionKv4Args &a, size_t quer
     *(uint2_t *)(a.output + query * a.output_stride + (size_t)head * a.cache.head_dim + d) = packed;
 }
 
-// Joins the sums of a workgroup's waves ([wave][row][dim]) and stores the rows.
-template <int kDim, int kRows, int kWaves>
+// Joins the sums of a workgroup's waves ([wave][row][kStride], a row's dims first) and stores the rows.
+template <int kDim, int kRows, int kWaves, int kStride>
 __device__ __forceinline__ void join_waves(const AttentionKv4Args &a, const RowTile &tile, int kv, int heads, const float2 (&bases)[kWaves][kRows], const float *sums) {
     constexpr int kParts = kDim / 4;  // float4s of a row
     for (int j = threadIdx.x; j < kRows * kParts; j += kWaves * kWave) {
@@ -252,7 +252,7 @@ __device__ __forceinline__ void join_waves(const AttentionKv4Args &a, const RowT
         for (int w = 0; w < kWaves; w++) {
             const float keep = __builtin_amdgcn_exp2f(bases[w][r].x - m);
             all += bases[w][r].y * keep;
-            o += *(const float4_t *)(sums + ((size_t)w * kRows + r) * kDim + d) * keep;
+            o += *(const float4_t *)(sums + ((size_t)w * kRows + r) * kStride + d) * keep;
         }
         const int at_row = tile.first_row + r;
         store_row(a, (size_t)(tile.row0 + at_row / heads), kv * heads + at_row % heads, d, o, all);
@@ -667,7 +667,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
         }
         if constexpr (kAlone) {
             __syncthreads();
-            join_waves<kDim, kRows, kWaves>(a, tile, kv, heads, join_bases, (const float *)lds_all);
+            join_waves<kDim, kRows, kWaves, kDim>(a, tile, kv, heads, join_bases, (const float *)lds_all);
             return;
         }
         left -= count;
@@ -696,6 +696,7 @@ struct Rows32 {
     static constexpr int kGroups = kDim / kKvGroup, kWords = kDim / 8;
     static constexpr int kRows = 32, kStep = 32;
     static constexpr int kLanesPerWord = 32 / kWords, kNibbles = 8 / kLanesPerWord;  // (kNibbles == kGroups: result tiles)
+    static constexpr int kJoinStride = kDim + 4;  // floats of a row in LDS: the lanes store the same dims of all rows at once
     struct Keys {
         uint4_t k[kGroups / 2];
         uint32_t scales[kGroups];
@@ -707,7 +708,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
     using R = Rows32<kDim>;
     constexpr int G = R::kGroups, kRows = R::kRows;
     constexpr bool kAlone = kWaves > 1;
-    __shared__ __align__(16) float join_sums[kAlone ? kWaves : 1][kAlone ? kRows : 1][kAlone ? kDim : 4];
+    __shared__ __align__(16) float join_sums[kAlone ? kWaves : 1][kAlone ? kRows : 1][kAlone ? R::kJoinStride : 4];
     __shared__ float2 join_bases[kAlone ? kWaves : 1][kRows];
     const Kv4Cache &c = a.cache;
     const int lane = threadIdx.x % kWave, half = lane >> 5, l32 = lane & 31;
@@ -942,7 +943,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
         }
         if constexpr (kAlone) {
             __syncthreads();
-            join_waves<kDim, kRows, kWaves>(a, tile, kv, heads, join_bases, (const float *)join_sums);
+            join_waves<kDim, kRows, kWaves, R::kJoinStride>(a, tile, kv, heads, join_bases, (const float *)join_sums);
             return;
         }
         left -= count;
