@@ -150,7 +150,7 @@ struct RowTile {
         pos0 = s.pos0;
         first_row = tile * rows_per_tile;
         rows_left = s.rows * heads >= plan.from_rows && s.rows * heads < plan.to_rows ? s.rows * heads - first_row : 0;
-        pos_low = s.pos0 + first_row / heads;
+        pos_low = max(s.pos0 + first_row / heads, -1);  // (rows before the first position see nothing; the largest window below -1 would wrap)
         pos_high = s.pos0 + (first_row + min(rows_left, rows_per_tile) - 1) / heads;
         const int lo = window_begin(a, pos_low), hi = min(pos_high + 1, position_limit(a));
         first_step = lo / step;
@@ -1091,7 +1091,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
             if (a.scale == 0) q[k] = half8_t{};
         }
         const int wave_rows = min(32, tile.rows_left - wave * 32);  // (none: the wave only helps with the tiles)
-        const int wave_low = tile.pos0 + (tile.first_row + wave * 32) / heads, wave_high = tile.pos0 + (tile.first_row + wave * 32 + max(wave_rows, 1) - 1) / heads;
+        const int wave_low = max(tile.pos0 + (tile.first_row + wave * 32) / heads, -1), wave_high = tile.pos0 + (tile.first_row + wave * 32 + max(wave_rows, 1) - 1) / heads;
 
         int held_from = first * P::kTile >> c.page_shift, held = table[min(held_from + lane, a.batch.width - 1)];
         struct Raw {

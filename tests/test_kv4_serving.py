@@ -135,6 +135,23 @@ def test_bounds_that_cut(torch_, rows, heads):
         assert (got[np.isnan(want)] == 7).all()
 
 
+@pytest.mark.parametrize("rows,heads", [(6, 1), (8, 1), (12, 4), (90, 1)])
+def test_the_widest_window(torch_, rows, heads):
+    """A window of 2^31 - 1 positions is none, also beside rows that lie before the first position."""
+    torch = torch_
+    rng = np.random.default_rng(rows)
+    cache, starts, lens, table = random_batch(rng, [rows - 4, 70], [rows, 4], 16, 1, 128)
+    q = up(torch, rng.standard_normal((rows + 4, heads, 128)).astype(np.float16))
+    dev, batch = on_device(torch, cache, starts, lens, table)
+    for bound in (100, 3000):
+        out = [torch.full_like(q, 7.0) for _ in range(2)]
+        for o, window in zip(out, (0, 2 ** 31 - 1)):
+            tl.attention_kv4(q, o, *dev, *batch, rows, bound, window=window)
+        assert torch.equal(out[0].view(torch.int16), out[1].view(torch.int16))
+    want, size, reach = plain.attend(cache, q.cpu().numpy(), starts, lens, table, 128 ** -0.5, 0)
+    check_attention(out[1].cpu().numpy(), want, size, reach, q)
+
+
 def test_shared_pages(torch_):
     """Two sequences with the same first pages, and one with a page twice."""
     torch = torch_
