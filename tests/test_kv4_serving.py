@@ -118,6 +118,44 @@ def test_not_finite(torch_, length, rows, heads, dim, window):
     check_attention(np.where(np.isnan(want), 0, got), np.where(np.isnan(want), 0, want), np.where(some, 0, size), np.nan_to_num(reach), q)
 
 
+@pytest.mark.parametrize("rows,heads,length", [(1, 4, 90), (1, 8, 90), (5, 4, 90), (40, 2, 90), (1, 4, 2500), (2, 4, 2500), (6, 4, 2500), (80, 1, 2500)])
+def test_queries_that_are_not_finite(torch_, rows, heads, length):
+    """They make their own row and head NaN and no other."""
+    torch = torch_
+    rng = np.random.default_rng(rows + heads + length)
+    cache, starts, lens, table = random_batch(rng, [length], [rows], 64, 1, 128)
+    q = rng.standard_normal((rows, heads, 128)).astype(np.float16)
+    dev, batch = on_device(torch, cache, starts, lens, table)
+    want, size, reach = plain.attend(cache, q, starts, lens, table, 128 ** -0.5, 0)
+    bad = np.zeros((rows, heads), bool)
+    bad[0, 0] = bad[rows // 2, heads - 1] = True
+    q[bad] = np.where(rng.integers(0, 2, (bad.sum(), 128)), np.inf, -np.inf)
+    q[bad, 3] = np.nan
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+    tl.attention_kv4(up(torch, q), out, *dev, *batch, rows, length)
+    got = out.cpu().numpy()
+    assert np.isnan(got[bad]).all() and np.isfinite(got[~bad]).all()
+    want[bad] = np.nan
+    check_attention(got, want, size, reach, q)
+
+
+@pytest.mark.parametrize("bound", [40, 5000])
+def test_many_sequences(torch_, bound):
+    """A thousand of them, of 0 to 40 positions, each its own row tile; and in line, tens in a wave's piece."""
+    torch = torch_
+    rng = np.random.default_rng(bound)
+    lengths = rng.integers(0, 41, 1000).tolist()
+    cache, starts, lens, table = random_batch(rng, lengths, [1] * 1000, 16, 1, 64)
+    q = rng.standard_normal((1000, 4, 64)).astype(np.float16)
+    dev, batch = on_device(torch, cache, starts, lens, table)
+    table_wide = torch.full((1000, 400), -1, dtype=torch.int32, device="cuda")
+    table_wide[:, :table.shape[1]] = batch[2]
+    want, size, reach = plain.attend(cache, q, starts, lens, table, 0.125, 0)
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda")
+    tl.attention_kv4(up(torch, q), out, *dev, batch[0], batch[1], table_wide, 1, bound)
+    check_attention(out.cpu().numpy(), want, size, reach, q)
+
+
 @pytest.mark.parametrize("rows,heads", [(6, 1), (6, 2), (12, 4), (90, 1)])
 def test_bounds_that_cut(torch_, rows, heads):
     """Rows from max_query on are left as they were; positions from max_length on count as absent."""
