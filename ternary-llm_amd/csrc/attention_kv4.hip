@@ -1424,7 +1424,12 @@ Plans plans_of(const AttentionKv4Args &a) {
         p.many_plan = RowPlan{0, (int)((rows + tile_rows - 1) / tile_rows), 1, 0, p.few ? kFewRows + 1 : 0, INT32_MAX};
         const long long tiles = (long long)a.batch.batch * p.many_plan.tiles;
         const int slots = 8 / p.many_waves * cus;  // two waves a SIMD
-        p.many_plan.alone = tiles * kv >= slots || (reach(a) + step - 1) / step <= 3;
+        // A row tile alone takes some 4.5 us per step of the longest; in line all steps are shared out evenly, and what a tile of 256
+        // rows leaves behind and its join cost some 32 us. (32 heads, 8 kv heads of 128, rows behind positions: 512 of 512 28 us
+        // alone and 43 in line, 1024 of 1024 43 and 63, 2048 of 2048 75 and 115; twice 512 of 2048 73 and 75; 512 of 2048 73 and
+        // 56, 100 of 2000 71 and 31.)
+        const long long steps = (reach(a) + step - 1) / step;
+        p.many_plan.alone = steps * (slots - tiles * kv) <= 7ll * slots;
         p.many_plan.workers = p.many_plan.alone ? (int)tiles : (slots + kv - 1) / kv;
         p.many_plan.least = 2;
         p.many_bytes = p.many_plan.alone ? 0 : Segments::bytes(a, p.many_plan, tile_rows);
@@ -1441,10 +1446,14 @@ template <int kDim, int kRows, int kStep>
 hipError_t launch_join(const AttentionKv4Args &a, const RowPlan &plan, size_t segments_at, hipStream_t s) {
     const unsigned tiles = (unsigned)(a.batch.batch * plan.tiles), kv = (unsigned)a.cache.n_kv_heads;
     const size_t lds = 16 * (size_t)plan.workers;  // a weight per row and part, of which there are at most `workers`
-    if ((long long)tiles * kv * (kRows / 4) < current_device_cus())
+    // 8 lanes a row and segment for few rows always, for more where the workgroups of kDim / 4 lanes would not give every CU one:
+    // 131 072 positions of one sequence 47.5 us with 8 and 52.1 with 32, 32 ragged users 33.4 and 34.0; 512 rows behind 9000
+    // positions, three times, 320 and 279, 64 rows behind 8192, 16 times, 116 and 108.
+    if (kRows <= 8 || (long long)tiles * kv * (kRows / 4) < current_device_cus()) {
         attention_join_kernel<kDim, kRows, kStep, 8><<<dim3(tiles, kv, kRows / 4 * (kDim / 32)), kJoinThreads, lds, s>>>(a, plan, segments_at);
-    else
-        attention_join_kernel<kDim, kRows, kStep, kDim / 4><<<dim3(tiles, kv, kRows / 4), kJoinThreads, lds, s>>>(a, plan, segments_at);
+        return hipGetLastError();
+    }
+    if constexpr (kRows > 8) attention_join_kernel<kDim, kRows, kStep, kDim / 4><<<dim3(tiles, kv, kRows / 4), kJoinThreads, lds, s>>>(a, plan, segments_at);
     return hipGetLastError();
 }
 
