@@ -371,8 +371,10 @@ def rotary(q, k, q_out, k_out, positions, rotary_dim, theta, layout="interleaved
     device), layout "interleaved" or "half", the first rotary_dim dims of each head, scaling "none", "linear", "ntk",
     "banded" or "yarn" (high_turns: 4 for "banded", 32 for "yarn" unless given). q, q_out: fp16 [rows, heads, dim], k, k_out
     [rows, kv_heads, dim] (or None), rows of any stride; the outputs may be the inputs."""
-    _want(layout in ROTARY_LAYOUTS, f"layout must be one of {sorted(ROTARY_LAYOUTS)}")
-    _want(scaling in ROTARY_SCALINGS, f"scaling must be one of {sorted(ROTARY_SCALINGS)}")
+    if layout not in ROTARY_LAYOUTS:
+        raise ValueError(f"layout must be one of {sorted(ROTARY_LAYOUTS)}")
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"scaling must be one of {sorted(ROTARY_SCALINGS)}")
     _want((k is None) == (k_out is None), "k and k_out come together")
     n, heads, dim = q.shape
     strides = [_rows(q, "q"), 0, _rows(q_out, "q_out"), 0]
