@@ -12,6 +12,7 @@
 #include <algorithm>
 
 #include "kv4.h"
+#include "kv4_rows.h"
 
 namespace tllm {
 namespace {
@@ -69,20 +70,7 @@ __device__ __forceinline__ float quad_max(float v) {
     return fmaxf(v, rotated<1>(v));
 }
 
-// Rows of a sequence, in range whatever the arrays hold.
-struct Sequence {
-    int row0, rows, pos0;  // first row, rows, position of the first row
-    __device__ Sequence(const AttentionKv4Args &a, int seq) {
-        const int s0 = a.batch.starts[seq], s1 = a.batch.starts[seq + 1];
-        row0 = s0;
-        rows = min(min(s1, a.batch.n_tokens) - s0, a.max_query);
-        if (s0 < 0) rows = 0;
-        const long long p = (long long)a.batch.lengths[seq] - s1 + s0;
-        pos0 = (int)max(min(p, (long long)INT32_MAX - (1 << 25)), -(1ll << 25));
-    }
-};
 __device__ __forceinline__ int position_limit(const AttentionKv4Args &a) { return min(a.batch.width << a.cache.page_shift, a.max_length); }
-__device__ __forceinline__ int window_begin(const AttentionKv4Args &a, int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; }
 
 // ------------------------------------------------------------------------------------------------- few rows: decode
 //
@@ -146,16 +134,16 @@ struct RowTile {
     __device__ RowTile(const AttentionKv4Args &a, const RowPlan &plan, int number, int rows_per_tile, int step) {
         const int seq = plan.tiles == 1 ? number : number / plan.tiles, tile = plan.tiles == 1 ? 0 : number - seq * plan.tiles;
         const int heads = a.n_heads / a.cache.n_kv_heads;
-        const Sequence s(a, seq);
+        const SequenceRows s = sequence_rows(a.batch.starts[seq], a.batch.starts[seq + 1], a.batch.lengths[seq], a.batch.n_tokens, a.max_query);
         row0 = s.row0;
         pos0 = s.pos0;
         first_row = tile * rows_per_tile;
-        rows_left = s.rows * heads >= plan.from_rows && s.rows * heads < plan.to_rows ? s.rows * heads - first_row : 0;
-        pos_low = max(s.pos0 + first_row / heads, -1);  // (rows before the first position see nothing; the largest window below -1 would wrap)
-        pos_high = s.pos0 + (first_row + min(rows_left, rows_per_tile) - 1) / heads;
-        const int lo = window_begin(a, pos_low), hi = min(pos_high + 1, position_limit(a));
-        first_step = lo / step;
-        steps = rows_left > 0 && hi > lo ? (hi + step - 1) / step - first_step : 0;
+        const TileSpan t = tile_span(s, first_row, heads, rows_per_tile, step, a.window, position_limit(a), plan.from_rows, plan.to_rows);
+        rows_left = t.rows_left;
+        pos_low = t.pos_low;
+        pos_high = t.pos_high;
+        first_step = t.first_step;
+        steps = t.steps;
     }
     RowTile() = default;
     __device__ RowTile of_lane(int lane) const {

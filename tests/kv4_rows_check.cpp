@@ -1,0 +1,67 @@
+// Host check of the rows and positions that the attention over the 4-bit cache takes from a batch's starts and lengths
+// (ternary-llm_amd/csrc/kv4_rows.h): whatever 32-bit words these are, rows lie in the row arrays, no arithmetic wraps (the build
+// traps on it), and a tile's steps are those that some row of it sees, worked out here in 64 bits.
+#include <algorithm>
+#include <climits>
+#include <cstdio>
+#include <random>
+#include <vector>
+
+#include "kv4_rows.h"
+
+using namespace tllm;
+typedef long long i64;
+
+static int bad = 0;
+#define CHECK(x) do { if (!(x)) { if (bad++ < 10) std::printf("line %d: %s\n", __LINE__, #x); } } while (0)
+
+static void check(int s0, int s1, int length, int n, int max_query, int heads, int window, int limit, int per_tile, int step, int from, int to) {
+    const SequenceRows s = sequence_rows(s0, s1, length, n, max_query);
+    const bool sound = s0 >= 0 && s0 < n && s1 > s0;
+    const i64 rows = sound ? std::min<i64>(std::min<i64>(s1, n) - s0, max_query) : 0;
+    CHECK(s.rows == rows && s.row0 >= 0 && (rows == 0 || (s.row0 == s0 && (i64)s.row0 + s.rows <= n)));
+    const i64 pos0 = (i64)length - s1 + s0;
+    if (rows) CHECK(s.pos0 == pos0 || (pos0 < -(1 << 25) && s.pos0 + rows < 0) || (pos0 > INT_MAX - (1 << 25) && s.pos0 > limit));
+    const i64 all = rows * heads;
+    const int tiles = (int)(((i64)std::min(max_query, n) * heads + per_tile - 1) / per_tile);
+    for (int tile = 0; tile < tiles; tile = tile < 3 || tile >= tiles - 2 ? tile + 1 : tiles - 2) {
+        const int first = tile * per_tile;
+        const TileSpan t = tile_span(s, first, heads, per_tile, step, window, limit, from, to);
+        const i64 left = all >= from && all < to ? std::max<i64>(all - first, 0) : 0;
+        CHECK(t.rows_left == left && t.steps >= 0 && t.first_step >= 0);
+        i64 lo = LLONG_MAX, hi = -1;  // positions that some row sees
+        for (i64 r = first; r < first + std::min<i64>(left, per_tile); r++) {
+            const i64 pos = s.pos0 + r / heads, a = window > 0 ? std::max<i64>(0, pos - window + 1) : 0, b = std::min<i64>(pos, (i64)limit - 1);
+            if (a <= b) lo = std::min(lo, a), hi = std::max(hi, b);
+        }
+        if (hi < 0) CHECK(t.steps == 0);
+        else CHECK((i64)t.first_step * step <= lo && ((i64)t.first_step + t.steps) * step > hi && ((i64)t.first_step + t.steps - 1) * step <= hi);
+    }
+}
+
+int main() {
+    std::mt19937 rng(7);
+    const int words[] = {INT_MIN, INT_MIN + 1, -3 * (1 << 29), -(1 << 30), -805306368, -(1 << 25), -256, -1, 0, 1, 2, 5, 16, 100, 255, 256, 1 << 20,
+                         (1 << 24) - 1, 1 << 25, 805306368, 1 << 30, 3 * (1 << 29), INT_MAX - 300, INT_MAX - 16, INT_MAX - 1, INT_MAX};
+    const auto any = [&](i64 low, i64 high) { return (int)(low + (i64)(rng() % (uint64_t)(high - low + 1))); };
+    const int tile_of[][2] = {{4, 64}, {8, 32}, {32, 32}, {256, 128}, {256, 256}};
+    for (const int s0 : words)
+        for (const int s1 : words)
+            for (const int length : words)
+                for (int i = 0; i < 12; i++) {
+                    const auto &shape = tile_of[rng() % 5];
+                    const int heads = any(1, 64), n = i & 1 ? any(1, 300) : any(1, (1 << 24) - 1);
+                    const int max_query = (int)std::min<i64>(n, std::min<i64>(any(1, 1 << 24), (1 << 27) / heads));
+                    const int window = i % 3 == 0 ? 0 : i % 3 == 1 ? any(1, 5000) : INT_MAX - any(0, 100);
+                    const int limit = any(1, 1 << 20);
+                    const int from = i % 5 == 0 ? 65 : 0, to = i % 5 == 1 ? 65 : INT_MAX;
+                    check(s0, s1, length, n, max_query, heads, window, limit, shape[0], shape[1], from, to);
+                }
+    for (int i = 0; i < 300000; i++) {  // any words, and sound ones
+        const auto &shape = tile_of[rng() % 5];
+        const int heads = any(1, 64), n = any(1, 2000), s0 = i & 1 ? (int)rng() : any(0, n), s1 = i & 1 ? (int)rng() : any(s0, n);
+        check(s0, s1, i & 2 ? (int)rng() : any(0, 5000), n, any(1, n), heads, i & 4 ? any(1, 4000) : 0, any(1, 6000), shape[0], shape[1], 0, INT_MAX);
+    }
+    std::printf("bad=%d\n", bad);
+    return bad != 0;
+}

@@ -1,0 +1,41 @@
+"""The attention over the 4-bit cache at the edges of what a call may hold: starts that are not ascending."""
+import numpy as np
+import pytest
+
+import ternary_llm_amd as tl
+from tests import kv4_plain as plain
+from tests.test_kv4 import check_attention, torch_, up  # noqa: F401
+from tests.test_kv4_serving import on_device, random_batch
+
+pytestmark = pytest.mark.gpu
+
+LOW, HIGH = -2 ** 31, 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("bound", [90, 5000])
+@pytest.mark.parametrize("max_query,heads", [(1, 4), (2, 4), (5, 4), (16, 4), (80, 1)])
+def test_starts_that_do_not_ascend(torch_, max_query, heads, bound):
+    """Sequences whose starts descend or lie out of range have no rows there: nothing but their rows inside the row arrays is
+    written, and the sequences beside them are what they would be."""
+    torch = torch_
+    rng = np.random.default_rng(max_query + heads + bound)
+    n, behind = max_query + 6, 40
+    cache, _, lens, table = random_batch(rng, [90] * 8, [1] * 8, 16, 1, 128)
+    q = rng.standard_normal((n + 2 * behind, heads, 128)).astype(np.float16)
+    dev, (_, dev_lens, dev_table) = on_device(torch, cache, np.zeros(1, np.int32), lens, table)
+    dev_q = up(torch, q)[behind:behind + n]
+    for middle in ([1 << 30, -3 * (1 << 29), 1, LOW, 1, 0, LOW], [805306368, 0, HIGH, LOW, HIGH, -1, 2], [n, n + 1, -5, n, 7, 7, 3],
+                   [HIGH, HIGH, LOW, LOW, 0, -1, HIGH]):
+        starts = np.array([0, max_query] + middle, np.int32)
+        claimed = np.zeros(n, int)
+        sound = [(0, max_query)]
+        for s0, s1 in zip(starts[:-1].tolist(), starts[1:].tolist()):
+            if 0 <= s0 < min(s1, n):
+                claimed[s0:min(s1, n, s0 + max_query)] += 1
+        out = torch.full((n + 2 * behind, heads, 128), 7.0, dtype=torch.float16, device="cuda")
+        tl.attention_kv4(dev_q, out[behind:behind + n], *dev, up(torch, starts), dev_lens, dev_table, max_query, bound)
+        got = out.cpu().numpy()
+        assert (got[:behind] == 7).all() and (got[behind + n:] == 7).all() and (got[behind:behind + n][claimed == 0] == 7).all()
+        want, size, reach = plain.attend(cache, q[behind:behind + n], sound[0], lens[:1], table[:1], 128 ** -0.5, 0)
+        want[claimed != 1] = np.nan
+        check_attention(got[behind:behind + n], want, size, reach, q)
