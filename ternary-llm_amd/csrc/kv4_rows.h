@@ -24,9 +24,9 @@ struct SequenceRows {
 // the row arrays have no rows (decided before any difference is taken: s1 - s0 may be any 33-bit number).
 TLLM_HD SequenceRows sequence_rows(int s0, int s1, int length, int n_tokens, int max_query) {
     if (s0 < 0 || s0 >= n_tokens || s1 <= s0) return SequenceRows{0, 0, 0};
-    // (rows are fewer than 2^24, so from -2^25 on none reaches position 0)
-    const long long pos = (long long)length - s1 + s0, top = INT32_MAX - (1 << 25), low = -(1 << 25);
-    return SequenceRows{s0, lower_of(lower_of(s1, n_tokens) - s0, max_query), (int)(pos < low ? low : pos > top ? top : pos)};
+    // (the last row's position is below `length`; rows are fewer than 2^24, so from -2^25 on none reaches position 0)
+    const long long pos = (long long)length - s1 + s0;
+    return SequenceRows{s0, lower_of(lower_of(s1, n_tokens) - s0, max_query), (int)(pos < -(1 << 25) ? -(1 << 25) : pos)};
 }
 
 // First position that a row at position pos (>= -1) sees.
@@ -47,9 +47,9 @@ TLLM_HD TileSpan tile_span(const SequenceRows &s, int first_row, int heads, int 
     t.rows_left = left;
     t.pos_low = higher_of(s.pos0 + first_row / heads, -1);  // (rows before the first position see nothing; the largest window below -1 would wrap)
     t.pos_high = s.pos0 + (first_row + lower_of(left, rows_per_tile) - 1) / heads;
-    const int lo = window_begin(window, t.pos_low), hi = lower_of(t.pos_high + 1, limit);
+    const int lo = window_begin(window, t.pos_low), hi = lower_of(t.pos_high, limit - 1);  // the last
     t.first_step = lo / step;
-    t.steps = hi > lo ? (hi + step - 1) / step - t.first_step : 0;
+    t.steps = hi >= lo ? hi / step - t.first_step + 1 : 0;
     return t;
 }
 

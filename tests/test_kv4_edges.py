@@ -1,4 +1,4 @@
-"""The attention over the 4-bit cache at the edges of what a call may hold: starts that are not ascending."""
+"""The attention over the 4-bit cache at the edges of what a call may hold: starts that are not ascending, positions near 2^31."""
 import numpy as np
 import pytest
 
@@ -39,3 +39,28 @@ def test_starts_that_do_not_ascend(torch_, max_query, heads, bound):
         want, size, reach = plain.attend(cache, q[behind:behind + n], sound[0], lens[:1], table[:1], 128 ** -0.5, 0)
         want[claimed != 1] = np.nan
         check_attention(got[behind:behind + n], want, size, reach, q)
+
+
+@pytest.mark.parametrize("rows,heads", [(1, 4), (2, 4), (5, 4), (80, 1)])
+def test_positions_near_two_to_the_31(torch_, rows, heads):
+    """The last positions that a page table can have, in a window: those of a short sequence with the same rows."""
+    torch = torch_
+    rng = np.random.default_rng(rows + heads)
+    page, held, width = 16, 13 * 16, (1 << 27) - 1
+    cache, starts, lens, table = random_batch(rng, [held], [rows], page, 1, 64)
+    q = up(torch, rng.standard_normal((rows, heads, 64)).astype(np.float16))
+    dev, batch = on_device(torch, cache, starts, lens, table)
+    far = torch.full((1, width), -1, dtype=torch.int32, device="cuda")
+    far[0, width - table.shape[1]:] = batch[2][0]
+    capacity = width * page
+    want, size, reach = plain.attend(cache, q.cpu().numpy(), starts, lens, table, 0.125, 50)
+    for bound in (capacity, HIGH):
+        out = torch.full_like(q, 7.0)
+        tl.attention_kv4(q, out, *dev, batch[0], up(torch, np.array([capacity], np.int32)), far, rows, bound, window=50)
+        check_attention(out.cpu().numpy(), want, size, reach, q)
+    # more positions than the table has: those behind it are not seen, and the window counts from the row
+    more = 20
+    out = torch.full_like(q, 7.0)
+    tl.attention_kv4(q, out, *dev, batch[0], up(torch, np.array([capacity + 14], np.int32)), far, rows, HIGH, window=50 + more)
+    moved, size, reach = plain.attend(cache, q.cpu().numpy(), starts, lens + 14, table, 0.125, 50 + more, max_length=held)
+    check_attention(out.cpu().numpy(), moved, size, reach, q)
