@@ -722,7 +722,8 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
     const int v_word = l32 % R::kWords, v_part = l32 / R::kWords;
     // this lane's bytes in 16 positions of a page
     const uint32_t key_offset = (uint32_t)((l32 & 15) * R::kWords + half * 2 * G) * 4, key_scale_offset = (uint32_t)(l32 & 15) * 4;
-    const uint32_t value_offset = (uint32_t)(half * R::kWords + v_word) * 16, value_scale_offset = (((uint32_t)(v_word / 4) << c.page_shift) + 4 * half) * 4;
+    const uint32_t value_offset = (uint32_t)(half * R::kWords + v_word) * 16;
+    const size_t value_scale_offset = (((size_t)(v_word / 4) << c.page_shift) + 4 * half) * 4;  // (the fourth group of the largest page: beyond 32 bits)
     const float to_log2 = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * (2.0f * 1.44269504088896f);
     // half of a code in fp16: 512 + c / 2 (32 + c / 2 from bits 4-7) less the rest
     uint32_t even_bits = 0x60006000u, odd_bits = 0x50005000u;  // (in registers: two constants make two instructions)
@@ -1098,7 +1099,8 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
         const int k_quad = lane & 3, k_pos = lane >> 2;
         const int v_block = lane & 3, v_word = G == 4 ? lane >> 2 : lane >> 2 & 7, v_part = G == 4 ? 0 : lane >> 5;
         const uint32_t k_offset = (uint32_t)(k_pos * P::kWords + k_quad * G) * 4, ks_offset = (uint32_t)k_pos * 4;
-        const uint32_t v_offset = (uint32_t)(v_block * 4 * P::kWords + v_word * 4) * 4, vs_offset = (((uint32_t)(v_word / 4) << c.page_shift) + v_block * 4) * 4;
+        const uint32_t v_offset = (uint32_t)(v_block * 4 * P::kWords + v_word * 4) * 4;
+        const size_t vs_offset = (((size_t)(v_word / 4) << c.page_shift) + v_block * 4) * 4;  // (the fourth group of the largest page: beyond 32 bits)
         const int slots = (1 << c.page_shift) - 1;
         auto load = [&](int step) {
             Raw x;

@@ -1,4 +1,5 @@
-"""The attention over the 4-bit cache at the edges of what a call may hold: starts that are not ascending, positions near 2^31."""
+"""The attention over the 4-bit cache at the edges of what a call may hold: starts that are not ascending, positions near 2^31,
+pages of 2^29 and 2^30 positions."""
 import numpy as np
 import pytest
 
@@ -64,3 +65,40 @@ def test_positions_near_two_to_the_31(torch_, rows, heads):
     tl.attention_kv4(q, out, *dev, batch[0], up(torch, np.array([capacity + 14], np.int32)), far, rows, HIGH, window=50 + more)
     moved, size, reach = plain.attend(cache, q.cpu().numpy(), starts, lens + 14, table, 0.125, 50 + more, max_length=held)
     check_attention(out.cpu().numpy(), moved, size, reach, q)
+
+
+@pytest.mark.parametrize("dim,page", [(128, 1 << 29), (64, 1 << 30)])
+def test_the_largest_pages(torch_, dim, page):
+    """One page whose groups of steps lie 2^31 and 2^32 bytes apart: rows at its beginning and at its end are those of a small cache."""
+    torch = torch_
+    need = page * dim + 4 * page * dim // 32 * 2
+    if torch.cuda.mem_get_info()[0] < need + (8 << 30):
+        pytest.skip("the card has no room for a page of this size")
+    scales = (1, 1, dim // 32, page, 2)
+    big = (torch.empty(1, 1, page, dim // 8, dtype=torch.int32, device="cuda"), torch.empty(scales, dtype=torch.float16, device="cuda"),
+           torch.empty(1, 1, page // 4, dim // 8, 4, dtype=torch.int32, device="cuda"), torch.empty(scales, dtype=torch.float16, device="cuda"))
+    int32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    small, rows = tl.kv4_cache(1, 512, 1, dim), 300
+    table = int32([0])
+    # (each group of its own size, so that another's step shows)
+    size = torch.tensor([1.0, 0.25, 4.0, 0.0625], device="cuda")[:dim // 32].repeat_interleave(32).half()
+    for at_end in (False, True):
+        gen = torch.Generator(device="cuda").manual_seed(dim)
+        k, v = (torch.randn(rows, 1, dim, dtype=torch.float16, device="cuda", generator=gen) * size for _ in range(2))
+        got = []
+        for cache, length in ((big, page if at_end else rows), (small, 512 if at_end else rows)):
+            batch = (int32(0, rows), int32(length), table)
+            tl.kv4_append(k, v, *cache, *batch)
+            ko, vo = torch.zeros_like(k), torch.zeros_like(v)
+            tl.kv4_read(ko, vo, *cache, *batch)
+            results = [ko, vo]
+            for n in (1, 2, 7, 100):
+                q = torch.randn(n, 4, dim, dtype=torch.float16, device="cuda", generator=torch.Generator(device="cuda").manual_seed(n))
+                o = torch.full_like(q, 7.0)
+                tl.attention_kv4(q, o, *cache, int32(0, n), int32(length), table, n, length, window=100)
+                results.append(o)
+            got.append(results)
+        for a, b in zip(*got):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+        k_read, v_read = got[1][:2]
+        assert ((v_read - v).abs() <= 0.6 * size).all() and ((k_read - k).abs() <= 0.6 * size).all()
