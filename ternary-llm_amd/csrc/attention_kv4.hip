@@ -671,6 +671,34 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
     }
 }
 
+// From 9 rows on k and v are brought to fp16, with one rounding and kept within its range, as kv4_read writes them: the code as
+// 1024 + c (64 + c from bits 4-7) less the rest, exactly, then c s + m. (Halves of s and m cannot overflow, but lose the last bits
+// of steps and minima below 2^-14: values of 1e-4 came out 4e-3 off.) m + 15 s may be half a step of s above fp16's largest
+// number; groups that are large enough for that (or not finite) show in one look at the exponents of s and m, and what becomes of
+// them then (kCut) is a piece of code of its own.
+constexpr uint32_t kEvenBits = 0x64006400u, kOddBits = 0x54005400u;
+// Bits 15 and 31 of what is added up with `or`: a step from 2^11 or a minimum from 2^15 on (15 * 2^11 + 2^15 < 65504), infinities and NaN.
+__device__ __forceinline__ uint32_t large_bits(uint32_t scale) { return (scale & 0x7C007C00u) + 0x08001800u; }
+constexpr uint32_t kLargeMask = 0x80008000u;
+// The compiler does not know that the words stay the same: what was made of them is made anew, not kept in registers for a rare branch.
+template <class T>
+__device__ __forceinline__ void anew(T &words) {
+    asm volatile("" : "+v"(words));
+}
+__device__ __forceinline__ bool not_finite(uint32_t scale) { return ((scale & 0x7C007C00u) + 0x04000400u) & 0x80008000u; }
+// Two values of the codes in `field` (under the even or the odd mask), whose group's steps and minima are s and m in each half.
+template <bool kCut>
+__device__ __forceinline__ uint32_t values_of(uint32_t field, bool odd, uint32_t bits, half2_t s, half2_t m) {
+    const half2_t code = __builtin_bit_cast(half2_t, (field & (odd ? kOddCodes : kEvenCodes)) | bits) - (odd ? half2_t{64, 64} : half2_t{1024, 1024});
+    half2_t x = __builtin_elementwise_fma(code, s, m);
+    if constexpr (kCut) {
+        // (the smaller of a number and NaN is the number: the limits of a group that is not finite are NaN too)
+        const half2_t none = __builtin_elementwise_fma(s, half2_t{0, 0}, m * half2_t{0, 0});
+        x = __builtin_elementwise_max(__builtin_elementwise_min(x, none + half2_t{65504, 65504}), none - half2_t{65504, 65504});
+    }
+    return __builtin_bit_cast(uint32_t, x);
+}
+
 // ------------------------------------------------------------------------------------------------- up to 32 rows a tile
 //
 // Bound: the vector pipe, which brings the cache to fp16: a position's 2 kDim values cost some eight instructions a wave, whatever
@@ -724,14 +752,10 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
     const uint32_t key_offset = (uint32_t)((l32 & 15) * R::kWords + half * 2 * G) * 4, key_scale_offset = (uint32_t)(l32 & 15) * 4;
     const uint32_t value_offset = (uint32_t)(half * R::kWords + v_word) * 16;
     const size_t value_scale_offset = (((size_t)(v_word / 4) << c.page_shift) + 4 * half) * 4;  // (the fourth group of the largest page: beyond 32 bits)
-    const float to_log2 = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * (2.0f * 1.44269504088896f);
-    // half of a code in fp16: 512 + c / 2 (32 + c / 2 from bits 4-7) less the rest
-    uint32_t even_bits = 0x60006000u, odd_bits = 0x50005000u;  // (in registers: two constants make two instructions)
+    const float to_log2 = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * 1.44269504088896f;
+    uint32_t even_bits = kEvenBits, odd_bits = kOddBits;  // (in registers: two constants make two instructions)
     asm("" : "+v"(even_bits), "+v"(odd_bits));
-    auto value2 = [&](uint32_t field, bool odd, half2_t s, half2_t m) {
-        const half2_t code = __builtin_bit_cast(half2_t, odd ? (field & kOddCodes) | odd_bits : (field & kEvenCodes) | even_bits) - (odd ? half2_t{32, 32} : half2_t{512, 512});
-        return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, s, m));
-    };
+    const auto value2 = [&](auto cut, uint32_t field, bool odd, half2_t s, half2_t m) { return values_of<cut.value>(field, odd, odd ? odd_bits : even_bits, s, m); };
 
     while (true) {
         const int count = min(tile.steps - offset, left);
@@ -811,21 +835,32 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
                 load_keys(next);
             }
             const bool whole = pages == 3 && first + R::kStep - 1 <= tile.pos_low && first + R::kStep <= limit && (a.window == 0 || first > tile.pos_high - a.window);
-            float16_t x = {};
+            float16_t x;
+            const auto scores = [&](auto cut) {
+                x = float16_t{};
 #pragma unroll
-            for (int quad = 0; quad < 2; quad++)
+                for (int quad = 0; quad < 2; quad++)
 #pragma unroll
-                for (int pair = 0; pair < G / 2; pair++) {
-                    const int word = quad * G + 2 * pair;
-                    const uint32_t w0 = now.k[word >> 2][word & 3], w1 = now.k[word >> 2][(word & 3) + 1];
+                    for (int pair = 0; pair < G / 2; pair++) {
+                        const int word = quad * G + 2 * pair;
+                        const uint32_t w0 = now.k[word >> 2][word & 3], w1 = now.k[word >> 2][(word & 3) + 1];
 #pragma unroll
-                    for (int odd = 0; odd < 2; odd++) {
-                        const half2_t both = __builtin_bit_cast(half2_t, now.scales[2 * pair + odd]) * half2_t{1, 0.5f};
-                        const half2_t s = {both[0], both[0]}, m = {both[1], both[1]};
-                        const uint4_t key = {value2(w0, odd, s, m), value2(w0 >> 8, odd, s, m), value2(w1, odd, s, m), value2(w1 >> 8, odd, s, m)};
-                        x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, key), q[(2 * pair + odd) * 2 + quad], x, 0, 0, 0);
+                        for (int odd = 0; odd < 2; odd++) {
+                            const half2_t both = __builtin_bit_cast(half2_t, now.scales[2 * pair + odd]), s = {both[0], both[0]}, m = {both[1], both[1]};
+                            const uint4_t key = {value2(cut, w0, odd, s, m), value2(cut, w0 >> 8, odd, s, m), value2(cut, w1, odd, s, m), value2(cut, w1 >> 8, odd, s, m)};
+                            x = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, key), q[(2 * pair + odd) * 2 + quad], x, 0, 0, 0);
+                        }
                     }
-                }
+            };
+            scores(std::false_type{});
+            uint32_t large = 0;
+#pragma unroll
+            for (int g = 0; g < G; g++) large |= large_bits(now.scales[g]);
+            if (__ballot(large & kLargeMask)) {
+#pragma unroll
+                for (int i = 0; i < G / 2; i++) anew(now.k[i]);
+                scores(std::true_type{});  // (again, with what is beyond fp16's range cut)
+            }
             if (!whole) {
                 asm volatile("");  // (a branch: not worked out and chosen from in every step)
 #pragma unroll
@@ -853,15 +888,41 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
             for (int j = 0; j < 16; j += 2)  // (of the rounded weights, which is what the values are multiplied with)
                 sum = __builtin_amdgcn_fdot2(half2_t{weights[j >> 3][j & 7], weights[j >> 3][(j & 7) + 1]}, half2_t{1, 1}, sum, false);
 
+            const auto weigh_values = [&](auto cut, const uint4_t (&scales)[4]) {
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    uint4_t values[R::kNibbles];
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const uint4_t words = v[2 * k + b], pairs = scales[2 * k + b];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const half2_t s = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(pairs[2 * j + 1], pairs[2 * j], 0x05040100u));
+                            const half2_t m = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(pairs[2 * j + 1], pairs[2 * j], 0x07060302u));
+#pragma unroll
+                            for (int byte = 0; byte < R::kNibbles / 2; byte++) {
+                                // this lane's byte `byte` of two positions' words, one per half
+                                const uint32_t which = (uint32_t)(v_part * (R::kNibbles / 2) + byte), select = which * 0x00010001u + 0x0C040C00u;
+                                const uint32_t field = __builtin_amdgcn_perm(words[2 * j + 1], words[2 * j], select);
+                                values[2 * byte][2 * b + j] = value2(cut, field, false, s, m);
+                                values[2 * byte + 1][2 * b + j] = value2(cut, field, true, s, m);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < R::kNibbles; n++) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, values[n]), weights[k], acc[n], 0, 0, 0);
+                }
+            };
             // what no row sees may be anything: its values are zeros (its weights are). So are groups that are not finite, and
             // the rows that see them get a NaN
-            uint32_t odd_one = 0;
+            large = 0;
 #pragma unroll
             for (int i = 0; i < 4; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) odd_one |= (v_scales[i][j] & 0x7C007C00u) + 0x04000400u;  // bits 15 and 31: an exponent is all ones
-            if (!whole || __ballot(odd_one & 0x80008000u)) {
-                asm volatile("");
+                for (int j = 0; j < 4; j++) large |= large_bits(v_scales[i][j]);
+            const bool any_large = __ballot(large & kLargeMask);
+            if (!whole || any_large) {
+                uint4_t cut[4] = {};  // steps and minima of the groups that are large: a product of their own
 #pragma unroll
                 for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -869,8 +930,10 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
                         const int t = first + 8 * i + j;  // (of the lower half of the lanes)
                         const int own = t + 4 * half;
                         const bool seen = (pages >> (i >> 1) & 1) && own <= tile.pos_high && own < limit && (a.window == 0 || own > tile.pos_low - a.window);
-                        const bool bad = seen && ((v_scales[i][j] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                        const bool bad = seen && not_finite(v_scales[i][j]);
                         v_scales[i][j] = seen && !bad ? v_scales[i][j] : 0;
+                        cut[i][j] = large_bits(v_scales[i][j]) & kLargeMask ? v_scales[i][j] : 0;
+                        v_scales[i][j] ^= cut[i][j];
                         const unsigned long long all_bad = __ballot(bad);
                         if (all_bad) {
                             for (int h = 0; h < 2; h++) {
@@ -887,30 +950,13 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
                             }
                         }
                     }
-            }
+                if (any_large) {
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                uint4_t values[R::kNibbles];
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    const uint4_t words = v[2 * k + b], pairs = v_scales[2 * k + b];
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        const half2_t s = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(pairs[2 * j + 1], pairs[2 * j], 0x05040100u));
-                        const half2_t m = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(pairs[2 * j + 1], pairs[2 * j], 0x07060302u)) * half2_t{0.5f, 0.5f};
-#pragma unroll
-                        for (int byte = 0; byte < R::kNibbles / 2; byte++) {
-                            // this lane's byte `byte` of two positions' words, one per half
-                            const uint32_t which = (uint32_t)(v_part * (R::kNibbles / 2) + byte), select = which * 0x00010001u + 0x0C040C00u;
-                            const uint32_t field = __builtin_amdgcn_perm(words[2 * j + 1], words[2 * j], select);
-                            values[2 * byte][2 * b + j] = value2(field, false, s, m);
-                            values[2 * byte + 1][2 * b + j] = value2(field, true, s, m);
-                        }
-                    }
+                    for (int i = 0; i < 4; i++) anew(v[i]);
+                    weigh_values(std::true_type{}, cut);
                 }
-#pragma unroll
-                for (int n = 0; n < R::kNibbles; n++) acc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, values[n]), weights[k], acc[n], 0, 0, 0);
             }
+            weigh_values(std::false_type{}, v_scales);
             now = next;
         }
 
@@ -919,7 +965,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
         const Segments segments(a, plan, kRows);
         const size_t place = ((size_t)kv * segments.per_head + worker + number) * kRows + l32;
         if (!entire && real && half == 0) *(float2 *)(segments.bases + place * 2) = make_float2(base, sum);
-        const float inv = sum == 0.0f ? 0.0f : 2.0f / sum;  // (half of v was taken); nothing seen: 0
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // nothing seen: 0
         if (kAlone || real) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
@@ -929,7 +975,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_rows_kernel(const 
 #pragma unroll
                 for (int n = 0; n < R::kNibbles; n += 2) {
                     if (!kAlone && entire) *(uint32_t *)(out + n) = (uint32_t)f2h(acc[n][e] * inv) | (uint32_t)f2h(acc[n + 1][e] * inv) << 16;
-                    else *(float2 *)(to + n) = make_float2(acc[n][e] * 2.0f, acc[n + 1][e] * 2.0f);
+                    else *(float2 *)(to + n) = make_float2(acc[n][e], acc[n + 1][e]);
                 }
             }
         }
@@ -1023,7 +1069,7 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(const Atte
 // while the tile before is worked on. 128 rows a workgroup took 211 us for a prompt of 4096 (32 heads, 8 kv heads of 128),
 // 256 take 171, 804 TFLOP/s of the seen half; a library's product of 8192^3 runs at 1177 on the card.
 // k and v are rounded to fp16 there, and p for the second product: three roundings of 2^-12 (root mean square) next to the
-// result's own; exact codes and two pieces of p, as for few rows, would cost as much again as all the rest. Half of k and v are stored: m + 15 s may be half a step of s above fp16's largest.
+// result's own; exact codes and two pieces of p, as for few rows, would cost as much again as all the rest.
 // v's rows of positions are stored with their 16-byte pieces exchanged by the row's eight (an exclusive or): the writes of a wave,
 // eight rows apart, would otherwise meet in two banks.
 // Transposed products (k q^T, v^T p^T) put a row's scores into one lane and its partner 32 lanes on, and p is then the next
@@ -1063,7 +1109,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
     const int limit = position_limit(a);
     const size_t code_words = kv4_code_words(1 << c.page_shift, kDim), scale_words = kv4_scale_words(1 << c.page_shift, kDim);
     // (the sign is the row operand's; a scale of 0 makes that 0, so that what is left out can stay at minus infinity)
-    const float to_log2 = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * (2.0f * 1.44269504088896f);
+    const float to_log2 = (a.scale == 0.0f ? 1.0f : fabsf(a.scale)) * 1.44269504088896f;
 
     while (true) {
         const int count = min(tile.steps - offset, left);
@@ -1135,47 +1181,54 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
             x.v_scales = *(const uint4_t *)(kBlocks == 2 && v_part ? vs_at[1] : vs_at[0]);
             return x;
         };
-        // codes 1024 + c (64 + c from bits 4-7) less the rest, times s / 2, plus m / 2
-        uint32_t even_bits = 0x64006400u, odd_bits = 0x54005400u;  // (in registers: two constants make two instructions)
+        uint32_t even_bits = kEvenBits, odd_bits = kOddBits;  // (in registers: two constants make two instructions)
         asm("" : "+v"(even_bits), "+v"(odd_bits));
-        auto value2 = [&](uint32_t field, bool odd, half2_t s, half2_t m) {
-            const half2_t code = __builtin_bit_cast(half2_t, odd ? (field & kOddCodes) | odd_bits : (field & kEvenCodes) | even_bits) - (odd ? half2_t{64, 64} : half2_t{1024, 1024});
-            return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(code, s, m));
-        };
+        const auto value2 = [&](auto cut, uint32_t field, bool odd, half2_t s, half2_t m) { return values_of<cut.value>(field, odd, odd ? odd_bits : even_bits, s, m); };
         auto store = [&](const Raw &x, int step, int into) {
             const int at = step * P::kTile;
             unsigned char *keys = stage[into], *values = stage[into] + P::kKeyTile;
+            const auto put_keys = [&](auto cut, const uint4_t &words) {
 #pragma unroll
-            for (int pair = 0; pair < 2; pair++) {
-                const uint32_t w0 = x.k[2 * pair], w1 = x.k[2 * pair + 1];
-                const int to = 16 * (wave + (G == 4 ? 0 : kWaves * pair)) + k_pos, group = G == 4 ? 2 * pair : 0;
+                for (int pair = 0; pair < 2; pair++) {
+                    const uint32_t w0 = words[2 * pair], w1 = words[2 * pair + 1];
+                    const int to = 16 * (wave + (G == 4 ? 0 : kWaves * pair)) + k_pos, group = G == 4 ? 2 * pair : 0;
 #pragma unroll
-                for (int odd = 0; odd < 2; odd++) {
-                    const half2_t both = __builtin_bit_cast(half2_t, x.k_scales[2 * pair + odd]) * half2_t{0.5f, 0.5f};
-                    const half2_t s = {both[0], both[0]}, m = {both[1], both[1]};
-                    const uint4_t out = {value2(w0, odd, s, m), value2(w0 >> 8, odd, s, m), value2(w1, odd, s, m), value2(w1 >> 8, odd, s, m)};
-                    *(uint4_t *)(keys + to * P::kKeyBytes + ((group + odd) * 32 + k_quad * 8) * 2) = out;
+                    for (int odd = 0; odd < 2; odd++) {
+                        const half2_t both = __builtin_bit_cast(half2_t, x.k_scales[2 * pair + odd]), s = {both[0], both[0]}, m = {both[1], both[1]};
+                        const uint4_t out = {value2(cut, w0, odd, s, m), value2(cut, w0 >> 8, odd, s, m), value2(cut, w1, odd, s, m), value2(cut, w1 >> 8, odd, s, m)};
+                        *(uint4_t *)(keys + to * P::kKeyBytes + ((group + odd) * 32 + k_quad * 8) * 2) = out;
+                    }
                 }
+            };
+            uint32_t large_key = 0, large = 0;
+#pragma unroll
+            for (int i = 0; i < 4; i++) large_key |= large_bits(x.k_scales[i]);
+            put_keys(std::false_type{}, x.k);
+            if (__ballot(large_key & kLargeMask)) {
+                uint4_t words = x.k;
+                anew(words);
+                put_keys(std::true_type{}, words);  // (again, with what is beyond fp16's range cut)
             }
             // what no row sees may be anything: its values are zeros (its scores are left out); so are the groups that are not
             // finite, which the rows that see them get from `unsound`
             const int part = wave + kWaves * v_part, from = at + 16 * part + v_block * 4;
-            uint32_t scales[4], odd_one = 0;
+            uint32_t scales[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 scales[j] = x.v_scales[j];
-                odd_one |= (scales[j] & 0x7C007C00u) + 0x04000400u;  // bits 15 and 31: an exponent is all ones
+                large |= large_bits(scales[j]);
             }
             // (positions of this step that all lie where some row sees them: all but the ends)
             const bool inside = x.there == (uint32_t)((1ull << (P::kTile / 16)) - 1) && at + P::kTile - 1 <= min(tile.pos_high, limit - 1) && (a.window == 0 || at > tile.pos_low - a.window);
-            if (!inside || __ballot(odd_one & 0x80008000u)) {
+            const bool any_large = __ballot(large & kLargeMask);
+            if (!inside || any_large) {
                 asm volatile("");
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int t = from + j;
                     const bool seen = (x.there >> part & 1) && t <= tile.pos_high && t < limit && (a.window == 0 || t > tile.pos_low - a.window);
                     const uint32_t w = scales[j];
-                    const bool bad = ((w & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                    const bool bad = not_finite(w);
                     if (seen && bad) {
                         atomicOr(&unsound[into][t - at], 1u << (v_word / 4));
                         unsound[into][P::kTile] = 1;
@@ -1186,19 +1239,27 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
             half2_t s[2], m[2];
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                s[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x05040100u)) * half2_t{0.5f, 0.5f};
-                m[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x07060302u)) * half2_t{0.5f, 0.5f};
+                s[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x05040100u));
+                m[j] = __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(scales[2 * j + 1], scales[2 * j], 0x07060302u));
             }
             unsigned char *to = values + v_word * 8 * P::kValueBytes + ((part * 32 + (v_block & 1) * 16) ^ (v_word & 15) << 4) + (v_block >> 1) * 8;
+            const auto put_values = [&](auto cut, const uint4_t &words) {
 #pragma unroll
-            for (int piece = 0; piece < 2; piece++) {
-                const uint32_t select = piece ? 0x07060302u : 0x05040100u;
-                const uint32_t p0 = __builtin_amdgcn_perm(x.v[1], x.v[0], select), p1 = __builtin_amdgcn_perm(x.v[3], x.v[2], select);
+                for (int piece = 0; piece < 2; piece++) {
+                    const uint32_t select = piece ? 0x07060302u : 0x05040100u;
+                    const uint32_t p0 = __builtin_amdgcn_perm(words[1], words[0], select), p1 = __builtin_amdgcn_perm(words[3], words[2], select);
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint2_t out = {value2(i & 2 ? p0 >> 8 : p0, i & 1, s[0], m[0]), value2(i & 2 ? p1 >> 8 : p1, i & 1, s[1], m[1])};
-                    *(uint2_t *)(to + (piece * 4 + i) * P::kValueBytes) = out;
+                    for (int i = 0; i < 4; i++) {
+                        const uint2_t out = {value2(cut, i & 2 ? p0 >> 8 : p0, i & 1, s[0], m[0]), value2(cut, i & 2 ? p1 >> 8 : p1, i & 1, s[1], m[1])};
+                        *(uint2_t *)(to + (piece * 4 + i) * P::kValueBytes) = out;
+                    }
                 }
+            };
+            put_values(std::false_type{}, x.v);
+            if (any_large) {
+                uint4_t words = x.v;
+                anew(words);
+                put_values(std::true_type{}, words);
             }
         };
 
@@ -1327,7 +1388,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
 
         sum += __shfl_xor(sum, 32, kWave);
         if (real) {
-            const float inv = sum == 0.0f ? 0.0f : 2.0f / sum;  // (half of v was stored); nothing seen: 0
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // nothing seen: 0
             const Segments segments(a, plan, P::kRows, segments_at);
             const size_t slot = ((size_t)kv * segments.per_head + worker + number) * P::kRows + in_tile;
             if (!entire && half == 0) *(float2 *)(segments.bases + slot * 2) = make_float2(base, sum);
@@ -1342,7 +1403,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
                         *(uint2_t *)(a.output + query * a.output_stride + (size_t)head * kDim + d) = packed;
                     } else {
                         *(float4_t *)(segments.sums + slot * kDim + d) =
-                            float4_t{acc[g][4 * j] * 2.0f, acc[g][4 * j + 1] * 2.0f, acc[g][4 * j + 2] * 2.0f, acc[g][4 * j + 3] * 2.0f};
+                            float4_t{acc[g][4 * j], acc[g][4 * j + 1], acc[g][4 * j + 2], acc[g][4 * j + 3]};
                     }
                 }
         }
