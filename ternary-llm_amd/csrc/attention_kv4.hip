@@ -6,9 +6,10 @@
 // subnormal c * 2^-24 (bits 0-3) or c * 2^-20 (bits 4-7), and v_mfma_f32_16x16x32_f16 takes subnormals as they are. 32 dims
 // are the depth of one such instruction, so one instruction sums one group; s and m are applied to its fp32 result. The
 // same holds for the values: sum_t p_t (m_tg + s_tg c_td) = sum_t (p_t s_tg) c_td + sum_t p_t m_tg with bare codes as one
-// operand and p s as the other. p s is taken in two fp16 pieces (the second is what the first's rounding left), so the only
-// roundings to fewer than 32 bits are 2^-22 of p s, and the result's. So up to 8 rows; more rows share keys and values that are
-// brought to fp16 once (the second and third kernel).
+// operand and p s as the other. p s is taken in two fp16 pieces (the second is what the first's rounding left), times a power of two
+// that follows the steps, or each row's and group's products (see kStepPower): the only roundings to fewer than 32 bits are 2^-22 of p s,
+// or 2^-29 of the largest of its row and group, and the result's. So up to 8 rows; more rows share keys and values that are brought to
+// fp16 once (the second and third kernel).
 #include <algorithm>
 
 #include "kv4.h"
@@ -21,13 +22,25 @@ typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
+typedef unsigned short ushort2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t uint4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t uint2_t __attribute__((ext_vector_type(2)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
 constexpr float kEmpty = -1e30f;  // below every score (|q.k| < 2^40, |scale| <= 2^40): no position yet
-constexpr int kHeadroom = 6;      // powers of two that a weight may outgrow its base by before everything is rescaled
-constexpr int kTopPower = 8;      // a base puts the largest weight seen (times its step) at 2^kTopPower
+constexpr int kHeadroom = 4;      // powers of two that a weight may outgrow its base by before everything is rescaled
+// What a weight times a step is multiplied by before it becomes fp16 (its lift) is a power of two. The steps of a group mostly lie within
+// a small factor of each other; then the largest of the first positions gives the group's lift: it comes to lie between
+// 2^(kStepPower - 1) and 2^kStepPower, and all steps of the piece have to lie between a 32nd of that and its double (a weight is at most
+// 2^kHeadroom: the products stay in fp16, whose pieces hold them to 2^-25). A row's largest product is then 2^4 at least. But the steps of
+// two positions may be any fp16 numbers apart, and one row look at the one and another row at the other (one lift for all lost 1.7 % of
+// the weights of steps of 2^-14 beside one of 8000). So a wave that meets other steps begins its piece again with a lift for each row and
+// group, by the products themselves: the largest so far came to lie between 2^(kTopPower - 1) and 2^kTopPower, taken anew where one
+// reaches 2^kLimitPower and raised where a new base leaves the earlier weights small. (Those in every piece from the start: 50.4 us for
+// 131 072 positions of one sequence, where this takes 47.6 if steps are alike; if none are, 76.)
+constexpr int kStepPower = 10, kTopPower = 10, kLimitPower = 15;
+constexpr int kMostLift = (127 + 32) << 23;  // 2^32 as a float's bits: the smallest step with a weight of 1 comes to 2^8, and what is lost is below 2^-57
+constexpr int kInverse = 254 << 23;          // less the bits of a power of two: those of its inverse
 constexpr uint32_t kEvenCodes = 0x000F000Fu, kOddCodes = 0x00F000F0u;
 // The values' codes are all brought to bits 4-7, and every second position's enter as 15 - c with a negative weight (15 p s
 // goes to the minima's sum). The matrix unit lines products up by their operands' exponents, of which a subnormal has the
@@ -62,6 +75,24 @@ __device__ __forceinline__ int running_sum(int v) {
     v += shifted<0x118, 0xF>(v);
     v += shifted<0x142, 0xA>(v);  // the last lane of quads 0 and 2 to quads 1 and 3
     return v + shifted<0x143, 0xC>(v);  // lane 31 to quads 2 and 3
+}
+__device__ __forceinline__ float as_float(int bits) { return __builtin_bit_cast(float, bits); }
+// The larger of two 16-bit halves each; over the lanes of a quad, in every lane; of a word of this half of the wave (kLanes 32; 16: of this
+// quad) and its partner, the even halves (quads) of the first word and the odd ones of the second.
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushort2_t, a), __builtin_bit_cast(ushort2_t, b)));
+}
+__device__ __forceinline__ uint32_t quad_larger(uint32_t v) {
+    const auto turned = [](uint32_t x, auto by) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x120 + by.value, 0xF, 0xF, false); };
+    v = larger(v, turned(v, std::integral_constant<int, 8>{}));
+    v = larger(v, turned(v, std::integral_constant<int, 4>{}));
+    v = larger(v, turned(v, std::integral_constant<int, 2>{}));
+    return larger(v, turned(v, std::integral_constant<int, 1>{}));
+}
+template <int kLanes>
+__device__ __forceinline__ uint32_t larger_of_swapped(uint32_t a, uint32_t b) {
+    const uint2_t both = kLanes == 32 ? __builtin_amdgcn_permlane32_swap(a, b, false, false) : __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    return larger(both[0], both[1]);
 }
 __device__ __forceinline__ float quad_max(float v) {
     v = fmaxf(v, rotated<8>(v));
@@ -286,6 +317,8 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
     const float sign = t16 & 1 ? -1.0f : 1.0f, flipped = t16 & 1 ? 15.0f : 0.0f;  // of this lane's positions
     float minus_one = -1.0f;  // (a variable: the product with it is folded into a mixed-precision instruction, a difference is not)
     asm("" : "+v"(minus_one));
+    // (with 4 rows a tile all lanes have the same rows: their lifts are the wave's)
+    const auto of_wave = [](int x) { return kRows == 4 ? __builtin_amdgcn_readfirstlane(x) : x; };
     const float c_low = a.scale * 1.44269504088896f, c_even = c_low * 16777216.0f, c_odd = c_low * 1048576.0f;
 
     while (true) {
@@ -386,208 +419,349 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
             }
         }
 
-        float4_t acc[D::kSets][D::kNibbles] = {};
-        float acc_min[G][4] = {}, sum[4] = {}, base[4] = {kEmpty, kEmpty, kEmpty, kEmpty};
-        int power = -24;          // 2^power is at least every step of the values seen so far
-        uint32_t power_bits = 0;  // ... as fp16 bits (steps are positive: their bits compare as the numbers do)
-
-        // this step's values, which the work on the scores covers, then the next step's keys
-        while (step < end) {
-            typename D::Values values;
-            load_values(values, at);
-            const uint32_t pages = at.there;
-            const int first = step * D::kStep;
-            typename D::Keys next;
-            step += kWaves;
-            if (step < end) {
-                at = find(step);
-                load_keys(next, at);
-            }
-            // whole: every row sees all of the step's positions
-            const bool whole = pages == (1u << D::kTiles) - 1 && first + D::kStep - 1 <= tile.pos_low && first + D::kStep <= limit &&
-                               (a.window == 0 || first > tile.pos_high - a.window);
-            float raw[4], most = -INFINITY;
-            uint32_t largest = 0, sees = ~0u;  // sees: a bit per row r
-            float4_t d[G];
+        float4_t acc[D::kSets][D::kNibbles];
+        float acc_min[G][4], sum[4], base[4];
+        int column_lift[D::kSets];  // of the column that this lane's sums of values belong to; lifts are the bits of their floats
+        // The piece's sums; with `each`, a lift for each row and group. False: the steps of some group are not alike.
+        const auto attend = [&](auto each) {
+            constexpr bool kEach = each.value;
 #pragma unroll
-            for (int pair = 0; pair < G / 2; pair++)
+            for (int e = 0; e < D::kSets; e++)
 #pragma unroll
-                for (int u = 0; u < D::kPack; u++) {
-                    const uint32_t w0 = now.k[u][2 * pair], w1 = now.k[u][2 * pair + 1];
-                    const uint4_t even = {w0 & kEvenCodes, w0 >> 8 & kEvenCodes, w1 & kEvenCodes, w1 >> 8 & kEvenCodes};
-                    const uint4_t odd = {w0 & kOddCodes, w0 >> 8 & kOddCodes, w1 & kOddCodes, w1 >> 8 & kOddCodes};
-                    const float4_t d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair], __builtin_bit_cast(half8_t, even), float4_t{}, 0, 0, 0);
-                    const float4_t d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair + 1], __builtin_bit_cast(half8_t, odd), float4_t{}, 0, 0, 0);
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        d[2 * pair][r] = u == 0 || pack == u ? d0[r] : d[2 * pair][r];
-                        d[2 * pair + 1][r] = u == 0 || pack == u ? d1[r] : d[2 * pair + 1][r];
-                    }
-                    if (u & 1) __builtin_amdgcn_sched_barrier(0);
-                }
-            bool unsound = false;
-            if (!whole) {
-                asm volatile("");  // (a branch: not worked out and chosen from in every step)
-                const int t = first + 16 * pack + t16;
-                const bool there = (pages >> pack & 1) && t < limit;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int row = 4 * row_quad + r, pos = tile.pos0 + (tile.first_row + row) / heads;
-                    const bool one = there && row < tile.rows_left && t <= pos && (a.window == 0 || t > pos - a.window);
-                    sees &= ~((uint32_t)!one << r);
-                }
-                // What no row sees may be anything, and must reach neither the powers below nor, in the product of the
-                // minima, the other tiles' positions. Nor must what is not finite and only some rows see reach the others:
-                // a key's rows get their NaN in the scores below, a value's in the sum of its group's minima.
-                const bool any = there && t <= tile.pos_high && (a.window == 0 || t > tile.pos_low - a.window);
-#pragma unroll
-                for (int g = 0; g < G; g++) {
-                    unsound |= any && (now.km[g] & 0x7C000000u) == 0x7C000000u;
-                    const bool wrong = any && ((now.vm[g] & 0x7C000000u) == 0x7C000000u || (now.vm[g] & 0x7C00u) == 0x7C00u);
-                    now.vm[g] = any && !wrong ? now.vm[g] : 0;
-#pragma unroll
-                    for (int r = 0; r < 4; r++) acc_min[g][r] = wrong && (sees >> r & 1) ? NAN : acc_min[g][r];
-                }
-#pragma unroll
-                for (int g = 0; g < G; g++) now.km[g] = any && !unsound ? now.km[g] : 0;
-            }
-            uint4_t minima;
-#pragma unroll
-            for (int j = 0; j < 4; j++)  // (G is 2: the last four depths have zero rows, and zeros here)
-                minima[j] = G == 4 || j < 2 ? __builtin_amdgcn_perm(now.km[2 * j % G + 1], now.km[2 * j % G], 0x07060302u) : 0;
-            const float4_t low = __builtin_amdgcn_mfma_f32_16x16x32_f16(q_sums, __builtin_bit_cast(half8_t, minima), float4_t{}, 0, 0, 0);
+                for (int i = 0; i < D::kNibbles; i++) acc[e][i] = float4_t{};
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                float even = 0, odd = 0;
+                sum[r] = 0;
+                base[r] = kEmpty;
 #pragma unroll
-                for (int g = 0; g < G; g += 2) {
-                    even = __builtin_fmaf(low_half(now.km[g]), d[g][r], even);
-                    odd = __builtin_fmaf(low_half(now.km[g + 1]), d[g + 1][r], odd);
-                }
-                raw[r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low[r] * (32.0f * c_low)));
+                for (int g = 0; g < G; g++) acc_min[g][r] = 0;
             }
-            if (!whole) {
-                asm volatile("");
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    raw[r] = unsound ? NAN : raw[r];
-                    raw[r] = sees >> r & 1 ? raw[r] : -INFINITY;
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) most = fmaxf(most, raw[r] - base[r]);
-#pragma unroll
-            for (int g = 0; g < G; g++) largest = max(largest, now.vm[g] & 0xFFFFu);
-            const bool grown = most > (float)(kHeadroom + kTopPower - power) || largest > power_bits;
-            if (__ballot(grown)) {
-                // rare after the first steps: new bases (a base is the row's largest score so far, moved by the powers)
-                int bits = (int)largest;
-#pragma unroll
-                for (int off = 1; off < kWave; off <<= 1) bits = max(bits, __shfl_xor(bits, off, kWave));
-                const float moved = (float)(power - kTopPower);
-                if ((uint32_t)bits > power_bits) {
-                    if (bits > 0x7BFF) bits = 0x7BFF;  // (infinite or NaN: the weights carry it on)
-                    int e;
-                    frexpf(h2f((uint16_t)bits), &e);  // steps <= 2^e
-                    power = e;
-                    power_bits = e > 15 ? 0x7BFFu : f2h(ldexpf(1.0f, e));
-                }
-                float keep[4];
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float m = quad_max(raw[r]);
-#pragma unroll
-                    for (int off = 4 * kRows; off < kWave; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
-                    const float to = fmaxf(base[r] - moved, m) + (float)(power - kTopPower);
-                    keep[r] = __builtin_amdgcn_exp2f(base[r] - to);
-                    base[r] = to;
-                    sum[r] *= keep[r];
-#pragma unroll
-                    for (int g = 0; g < G; g++) acc_min[g][r] *= keep[r];
-                }
-                const int row = t16 % kRows;
-                float column = 0;
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float k = __shfl(keep[r], (row >> 2) * 16, kWave);
-                    column = (row & 3) == r ? k : column;
-                }
-#pragma unroll
-                for (int e = 0; e < D::kSets; e++)
-#pragma unroll
-                    for (int i = 0; i < D::kNibbles; i++) acc[e][i] *= column;
-            }
-            float w[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                w[r] = __builtin_amdgcn_exp2f(raw[r] - base[r]);
-                sum[r] += w[r];
-            }
-            unsigned char *to = lds + (16 * pack + t16) * D::kRowBytes + row_quad * 8;
+            bool fresh = true, alike = true;           // (one lift a group:) no step of a value has been met; they are alike so far
+            int stop = end;                            // (one way out of the loop: a second costs copies of all sums in every step)
+            int group_lift[G], lift[kEach ? G : 1][4];  // of the groups; of this lane's rows (4 rows a tile: of the wave's)
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                const float size = low_half(now.vm[g]) * sign, low = __builtin_fmaf(low_half(now.vm[g]), flipped, high_half(now.vm[g]));
-                float ws[4];
-                uint32_t hi[2], lo[2];
+                group_lift[g] = kMostLift;
+#pragma unroll
+                for (int r = 0; r < 4; r++) lift[kEach ? g : 0][r] = kMostLift;
+            }
+#pragma unroll
+            for (int e = 0; e < D::kSets; e++) column_lift[e] = kMostLift;
+            // a column's new lift, and its sums under it
+            const auto change_column = [&](int e, int to) {
+                const float by = as_float(to) * as_float(kInverse - column_lift[e]);
+                column_lift[e] = to;
+#pragma unroll
+                for (int i = 0; i < D::kNibbles; i++) acc[e][i] *= by;
+            };
+
+            // this step's values, which the work on the scores covers, then the next step's keys
+            while (step < stop) {
+                typename D::Values values;
+                load_values(values, at);
+                const uint32_t pages = at.there;
+                const int first = step * D::kStep;
+                typename D::Keys next;
+                step += kWaves;
+                if (step < end) {
+                    at = find(step);
+                    load_keys(next, at);
+                }
+                // whole: every row sees all of the step's positions
+                const bool whole = pages == (1u << D::kTiles) - 1 && first + D::kStep - 1 <= tile.pos_low && first + D::kStep <= limit &&
+                                   (a.window == 0 || first > tile.pos_high - a.window);
+                float raw[4], most = -INFINITY;
+                uint32_t sees = ~0u;  // a bit per row r
+                bool any = true;      // some row may see this lane's position
+                float4_t d[G];
+#pragma unroll
+                for (int pair = 0; pair < G / 2; pair++)
+#pragma unroll
+                    for (int u = 0; u < D::kPack; u++) {
+                        const uint32_t w0 = now.k[u][2 * pair], w1 = now.k[u][2 * pair + 1];
+                        const uint4_t even = {w0 & kEvenCodes, w0 >> 8 & kEvenCodes, w1 & kEvenCodes, w1 >> 8 & kEvenCodes};
+                        const uint4_t odd = {w0 & kOddCodes, w0 >> 8 & kOddCodes, w1 & kOddCodes, w1 >> 8 & kOddCodes};
+                        const float4_t d0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair], __builtin_bit_cast(half8_t, even), float4_t{}, 0, 0, 0);
+                        const float4_t d1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(q[2 * pair + 1], __builtin_bit_cast(half8_t, odd), float4_t{}, 0, 0, 0);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            d[2 * pair][r] = u == 0 || pack == u ? d0[r] : d[2 * pair][r];
+                            d[2 * pair + 1][r] = u == 0 || pack == u ? d1[r] : d[2 * pair + 1][r];
+                        }
+                        if (u & 1) __builtin_amdgcn_sched_barrier(0);
+                    }
+                bool unsound = false;
+                if (!whole) {
+                    asm volatile("");  // (a branch: not worked out and chosen from in every step)
+                    const int t = first + 16 * pack + t16;
+                    const bool there = (pages >> pack & 1) && t < limit;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int row = 4 * row_quad + r, pos = tile.pos0 + (tile.first_row + row) / heads;
+                        const bool one = there && row < tile.rows_left && t <= pos && (a.window == 0 || t > pos - a.window);
+                        sees &= ~((uint32_t)!one << r);
+                    }
+                    // What no row sees may be anything, and must reach neither the powers below nor, in the product of the
+                    // minima, the other tiles' positions. Nor must what is not finite and only some rows see reach the others:
+                    // a key's rows get their NaN in the scores below, a value's in the sum of its group's minima.
+                    any = there && t <= tile.pos_high && (a.window == 0 || t > tile.pos_low - a.window);
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        unsound |= any && (now.km[g] & 0x7C000000u) == 0x7C000000u;
+                        const bool wrong = any && ((now.vm[g] & 0x7C000000u) == 0x7C000000u || (now.vm[g] & 0x7C00u) == 0x7C00u);
+                        now.vm[g] = any && !wrong ? now.vm[g] : 0;
+#pragma unroll
+                        for (int r = 0; r < 4; r++) acc_min[g][r] = wrong && (sees >> r & 1) ? NAN : acc_min[g][r];
+                    }
+#pragma unroll
+                    for (int g = 0; g < G; g++) now.km[g] = any && !unsound ? now.km[g] : 0;
+                }
+                uint4_t minima;
+#pragma unroll
+                for (int j = 0; j < 4; j++)  // (G is 2: the last four depths have zero rows, and zeros here)
+                    minima[j] = G == 4 || j < 2 ? __builtin_amdgcn_perm(now.km[2 * j % G + 1], now.km[2 * j % G], 0x07060302u) : 0;
+                const float4_t low = __builtin_amdgcn_mfma_f32_16x16x32_f16(q_sums, __builtin_bit_cast(half8_t, minima), float4_t{}, 0, 0, 0);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    ws[r] = w[r] * size;
-                    acc_min[g][r] = __builtin_fmaf(w[r], low, acc_min[g][r]);
-                }
+                    float even = 0, odd = 0;
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const half2_t h = {(_Float16)ws[2 * j], (_Float16)ws[2 * j + 1]};
-                    const half2_t l = {(_Float16)__builtin_fmaf((float)h[0], minus_one, ws[2 * j]), (_Float16)__builtin_fmaf((float)h[1], minus_one, ws[2 * j + 1])};
-                    hi[j] = __builtin_bit_cast(uint32_t, h);
-                    lo[j] = __builtin_bit_cast(uint32_t, l);
-                }
-                *(uint2_t *)(to + g * kRows * 2) = uint2_t{hi[0], hi[1]};
-                *(uint2_t *)(to + D::kColumns * 2 + g * kRows * 2) = uint2_t{lo[0], lo[1]};
-            }
-            // (the lanes read each other's weights: the wave's LDS accesses run in order, the compiler has to keep it)
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll
-            for (int half = 0; half < D::kTiles / 2; half++) {
-                half8_t weights[D::kSets][2];
-#pragma unroll
-                for (int e = 0; e < D::kSets; e++)
-#pragma unroll
-                    for (int piece = 0; piece < 2; piece++) {
-                        short4_t two[2];
-#pragma unroll
-                        for (int i = 0; i < 2; i++) {
-                            unsigned char *from = lds + (16 * (2 * half + i) + 4 * quad + (lane >> 2 & 3)) * D::kRowBytes + piece * D::kColumns * 2 + e * 32 + (lane & 3) * 8;
-                            two[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)from);
-                        }
-                        struct Both { short4_t x[2]; } both = {{two[0], two[1]}};
-                        weights[e][piece] = __builtin_bit_cast(half8_t, both);
+                    for (int g = 0; g < G; g += 2) {
+                        even = __builtin_fmaf(low_half(now.km[g]), d[g][r], even);
+                        odd = __builtin_fmaf(low_half(now.km[g + 1]), d[g + 1][r], odd);
                     }
+                    raw[r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low[r] * (32.0f * c_low)));
+                }
+                if (!whole) {
+                    asm volatile("");
 #pragma unroll
-                for (int e = 0; e < D::kSets; e++) {
-                    const uint4_t va = values.v[2 * half][e], vb = values.v[2 * half + 1][e];
-#pragma unroll
-                    for (int byte = 0; byte < D::kNibbles / 2; byte++) {
-                        // this lane's byte `byte` of two positions' words, one per half
-                        const uint32_t which = (uint32_t)(t16 % D::kLanesPerWord * (D::kNibbles / 2) + byte), select = which * 0x00010001u + 0x0C040C00u;
-                        const uint32_t pairs[4] = {__builtin_amdgcn_perm(va[1], va[0], select), __builtin_amdgcn_perm(va[3], va[2], select),
-                                                   __builtin_amdgcn_perm(vb[1], vb[0], select), __builtin_amdgcn_perm(vb[3], vb[2], select)};
-#pragma unroll
-                        for (int odd = 0; odd < 2; odd++) {
-                            uint4_t codes;
-#pragma unroll
-                            for (int j = 0; j < 4; j++) codes[j] = ((odd ? pairs[j] : pairs[j] << 4) ^ kSecondFlipped) & kOddCodes;
-                            float4_t &into = acc[e][2 * byte + odd];
-                            into = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes), weights[e][0], into, 0, 0, 0);
-                            into = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes), weights[e][1], into, 0, 0, 0);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
+                    for (int r = 0; r < 4; r++) {
+                        raw[r] = unsound ? NAN : raw[r];
+                        raw[r] = sees >> r & 1 ? raw[r] : -INFINITY;
                     }
                 }
+#pragma unroll
+                for (int r = 0; r < 4; r++) most = fmaxf(most, raw[r] - base[r]);
+                float size[G];  // steps times their group's lift; odd positions' are negative (see kSecondFlipped)
+                if constexpr (!kEach) {
+                    if (fresh) {
+                        uint32_t steps[G / 2];  // of two groups
+#pragma unroll
+                        for (int i = 0; i < G / 2; i++) steps[i] = __builtin_amdgcn_perm(now.vm[2 * i + 1], now.vm[2 * i], 0x05040100u);
+                        uint32_t highest = larger_of_swapped<32>(steps[0], steps[G / 2 - 1]);  // halves of the wave: of these two
+                        highest = quad_larger(larger_of_swapped<16>(highest, highest));
+                        fresh = !__ballot(highest);
+#pragma unroll
+                        for (int g = 0; g < G; g++) {
+                            const int one = __builtin_amdgcn_readlane(highest, g / 2 * 32) >> g % 2 * 16 & 0xFFFF;
+                            group_lift[g] = one ? (127 + kStepPower + 14 - (one >> 10)) << 23 : kMostLift;
+                        }
+                    }
+                    float most_size = 0, least_size = INFINITY;
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        size[g] = low_half(now.vm[g]) * (as_float(group_lift[g]) * sign);
+                        most_size = fmaxf(most_size, fabsf(size[g]));
+                        least_size = fminf(least_size, fabsf(size[g]));
+                    }
+                    if (__ballot(any && (most_size > (float)(2 << kStepPower) || least_size < (float)(1 << kStepPower >> 5)))) stop = step, alike = false;
+                } else {
+#pragma unroll
+                    for (int g = 0; g < G; g++) size[g] = low_half(now.vm[g]) * sign;
+                }
+                if (__ballot(most > (float)kHeadroom)) {
+                    // rare after the first steps: new bases, whole numbers, so that what they change are powers of two
+                    float keep[4];
+                    int more[4];  // powers of two, as a float's bits, that the lifts are raised by
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        float m = quad_max(raw[r]);
+#pragma unroll
+                        for (int off = 4 * kRows; off < kWave; off <<= 1) m = fmaxf(m, __shfl_xor(m, off, kWave));
+                        const float to = fmaxf(base[r], ceilf(m));
+                        keep[r] = __builtin_amdgcn_exp2f(base[r] - to);
+                        more[r] = of_wave((int)fminf(to - base[r], 64.0f) << 23);
+                        base[r] = to;
+                        sum[r] *= keep[r];
+#pragma unroll
+                        for (int g = 0; g < G; g++) acc_min[g][r] *= keep[r];
+                    }
+                    const int row = t16 % kRows;
+                    float column = 0;
+                    int column_more = 0;
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const float k = kRows == 4 ? keep[r] : __shfl(keep[r], (row >> 2) * 16, kWave);
+                        column = (row & 3) == r ? k : column;
+                        if constexpr (kEach) {
+                            const int one = kRows == 4 ? more[r] : __shfl(more[r], (row >> 2) * 16, kWave);
+                            column_more = (row & 3) == r ? one : column_more;
+#pragma unroll
+                            for (int g = 0; g < G; g++) lift[g][r] = min(lift[g][r] + more[r], kMostLift);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < D::kSets; e++) {
+#pragma unroll
+                        for (int i = 0; i < D::kNibbles; i++) acc[e][i] *= column;
+                        if constexpr (kEach) change_column(e, min(column_lift[e] + column_more, kMostLift));
+                    }
+                }
+                float w[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    w[r] = __builtin_amdgcn_exp2f(raw[r] - base[r]);
+                    sum[r] += w[r];
+                }
+                // the weights of all groups in two pieces; the larger of the first pieces' bits (a lane's all have one sign)
+                const auto put_weights = [&] {
+                    unsigned char *to = lds + (16 * pack + t16) * D::kRowBytes + row_quad * 8;
+                    ushort2_t high = {0, 0};
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        uint32_t hi[2], lo[2];
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            float one = w[2 * j] * size[g], two = w[2 * j + 1] * size[g];
+                            if constexpr (kEach) one *= as_float(lift[g][2 * j]), two *= as_float(lift[g][2 * j + 1]);
+                            const half2_t h = {(_Float16)one, (_Float16)two};
+                            const half2_t l = {(_Float16)__builtin_fmaf((float)h[0], minus_one, one), (_Float16)__builtin_fmaf((float)h[1], minus_one, two)};
+                            hi[j] = __builtin_bit_cast(uint32_t, h);
+                            lo[j] = __builtin_bit_cast(uint32_t, l);
+                            high = __builtin_elementwise_max(high, __builtin_bit_cast(ushort2_t, h));
+                        }
+                        *(uint2_t *)(to + g * kRows * 2) = uint2_t{hi[0], hi[1]};
+                        *(uint2_t *)(to + D::kColumns * 2 + g * kRows * 2) = uint2_t{lo[0], lo[1]};
+                    }
+                    return __builtin_bit_cast(uint32_t, high);
+                };
+                if constexpr (!kEach) {
+                    put_weights();
+                } else if (__ballot(((put_weights() & 0x7FFF7FFFu) + 0x00010001u * (0x8000u - ((15u + kLimitPower) << 10))) & 0x80008000u)) {
+                    // (bits 15 and 31: an exponent of kLimitPower or more.) Lifts by the largest products, of which the exponents are enough: the
+                    // upper halves of two rows' in a word
+                    uint32_t high[2 * G];  // [2 g + j]: group g, rows 2 j and 2 j + 1
+#pragma unroll
+                    for (int g = 0; g < G; g++)
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const float size = fabsf(low_half(now.vm[g]));
+                            high[2 * g + j] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, w[2 * j + 1] * size), __builtin_bit_cast(uint32_t, w[2 * j] * size), 0x07060302u);
+                        }
+                    const auto new_lift = [](int old, uint32_t pair, bool second) {
+                        const int power = (int)(pair >> (second ? 23 : 7) & 0xFF);  // (infinite or NaN, 255: the weights carry it on)
+                        return (old >> 23) + power < 254 + kLimitPower ? old : (253 + kTopPower - power) << 23;
+                    };
+                    // swapping halves of the wave between two words and taking the larger leaves each half with one word's: [k] and [k + G]
+#pragma unroll
+                    for (int k = 0; k < G; k++) high[k] = larger_of_swapped<32>(high[k], high[k + G]);
+                    const int row = t16 % kRows;
+                    if constexpr (kRows == 4) {
+                        // the same with quads: quad n has words n * G / 2 + k
+#pragma unroll
+                        for (int k = 0; k < G / 2; k++) high[k] = quad_larger(larger_of_swapped<16>(high[k], high[k + G / 2]));
+#pragma unroll
+                        for (int n = 0; n < 2 * G; n++) {
+                            const uint32_t pair = __builtin_amdgcn_readlane(high[n % (G / 2)], n / (G / 2) * 16);
+#pragma unroll
+                            for (int i = 0; i < 2; i++) lift[n / 2][2 * (n & 1) + i] = new_lift(lift[n / 2][2 * (n & 1) + i], pair, i);
+                        }
+                        // this lane's column: group t16 / 4 (or none), word 2 * group + row / 2
+                        const int word = 2 * (t16 / 4 % G) + (row >> 1);
+                        uint32_t pair = __shfl(high[0], word / (G / 2) * 16, kWave);
+                        if constexpr (G == 4) {
+                            const uint32_t odd = __shfl(high[1], word / 2 * 16, kWave);
+                            pair = word & 1 ? odd : pair;
+                        }
+                        change_column(0, new_lift(column_lift[0], pair, row & 1));
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < G; k++) {
+                            high[k] = quad_larger(high[k]);
+                            const uint2_t both = __builtin_amdgcn_permlane32_swap(high[k], high[k], false, false);
+                            high[k] = both[0];
+                            high[k + G] = both[1];
+                        }
+#pragma unroll
+                        for (int n = 0; n < 2 * G; n++)
+#pragma unroll
+                            for (int i = 0; i < 2; i++) lift[n / 2][2 * (n & 1) + i] = new_lift(lift[n / 2][2 * (n & 1) + i], high[n], i);
+#pragma unroll
+                        for (int e = 0; e < D::kSets; e++) {
+                            uint32_t pair = 0;
+#pragma unroll
+                            for (int n = 0; n < 2 * D::kSetGroups; n++) {
+                                const uint32_t one = __shfl(high[2 * e * D::kSetGroups + n], (row >> 2) * 16, kWave);
+                                pair = n == 2 * (t16 / kRows) + (row >> 1 & 1) ? one : pair;
+                            }
+                            change_column(e, new_lift(column_lift[e], pair, row & 1));
+                        }
+                    }
+                    put_weights();
+                }
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    const float low = __builtin_fmaf(low_half(now.vm[g]), flipped, high_half(now.vm[g]));
+#pragma unroll
+                    for (int r = 0; r < 4; r++) acc_min[g][r] = __builtin_fmaf(w[r], low, acc_min[g][r]);
+                }
+                // (the lanes read each other's weights: the wave's LDS accesses run in order, the compiler has to keep it)
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int half = 0; half < D::kTiles / 2; half++) {
+                    half8_t weights[D::kSets][2];
+#pragma unroll
+                    for (int e = 0; e < D::kSets; e++)
+#pragma unroll
+                        for (int piece = 0; piece < 2; piece++) {
+                            short4_t two[2];
+#pragma unroll
+                            for (int i = 0; i < 2; i++) {
+                                unsigned char *from = lds + (16 * (2 * half + i) + 4 * quad + (lane >> 2 & 3)) * D::kRowBytes + piece * D::kColumns * 2 + e * 32 + (lane & 3) * 8;
+                                two[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t *)from);
+                            }
+                            struct Both { short4_t x[2]; } both = {{two[0], two[1]}};
+                            weights[e][piece] = __builtin_bit_cast(half8_t, both);
+                        }
+#pragma unroll
+                    for (int e = 0; e < D::kSets; e++) {
+                        const uint4_t va = values.v[2 * half][e], vb = values.v[2 * half + 1][e];
+#pragma unroll
+                        for (int byte = 0; byte < D::kNibbles / 2; byte++) {
+                            // this lane's byte `byte` of two positions' words, one per half
+                            const uint32_t which = (uint32_t)(t16 % D::kLanesPerWord * (D::kNibbles / 2) + byte), select = which * 0x00010001u + 0x0C040C00u;
+                            const uint32_t pairs[4] = {__builtin_amdgcn_perm(va[1], va[0], select), __builtin_amdgcn_perm(va[3], va[2], select),
+                                                       __builtin_amdgcn_perm(vb[1], vb[0], select), __builtin_amdgcn_perm(vb[3], vb[2], select)};
+#pragma unroll
+                            for (int odd = 0; odd < 2; odd++) {
+                                uint4_t codes;
+#pragma unroll
+                                for (int j = 0; j < 4; j++) codes[j] = ((odd ? pairs[j] : pairs[j] << 4) ^ kSecondFlipped) & kOddCodes;
+                                float4_t &into = acc[e][2 * byte + odd];
+                                into = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes), weights[e][0], into, 0, 0, 0);
+                                into = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, codes), weights[e][1], into, 0, 0, 0);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+                now = next;
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            now = next;
+            if constexpr (!kEach)
+#pragma unroll
+                for (int g = 0; g < G; g++)
+                    if (g % D::kSetGroups == 0 || t16 / kRows == g % D::kSetGroups) column_lift[g / D::kSetGroups] = group_lift[g];
+            return alike;
+        };
+        if (!attend(std::false_type{})) {
+            step = tile.first_step + offset + wave;
+            held_from = (tile.first_step + offset) * D::kStep >> c.page_shift;
+            held = table[min(held_from + lane, a.batch.width - 1)];
+            at = find(step);
+            load_keys(now, at);
+            attend(std::true_type{});
         }
 
         // ---- the sums of weights and minima over the lanes: inside each quad, then through LDS. A lane's results are column
@@ -637,7 +811,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
                     const int d = (e * D::kSetWords + n / D::kLanesPerWord) * 8 + n % D::kLanesPerWord * D::kNibbles;
                     float v[D::kNibbles];
 #pragma unroll
-                    for (int i = 0; i < D::kNibbles; i++) v[i] = __builtin_fmaf(acc[e][i][r], 1048576.0f, low[e]);
+                    for (int i = 0; i < D::kNibbles; i++) v[i] = __builtin_fmaf(acc[e][i][r], 1048576.0f * as_float(kInverse - column_lift[e]), low[e]);
                     if constexpr (kAlone) {
                         float *to = (float *)lds_all + ((size_t)wave * kRows + row) * kDim + d;
 #pragma unroll

@@ -62,3 +62,83 @@ def test_values_at_the_end_of_fp16(torch_, rows, heads, bound):
         np.testing.assert_array_equal(np.isnan(got), np.isnan(want))
         bad = np.isnan(want)
         check_attention(np.where(bad, 0, got), np.where(bad, 0, want), np.where(bad, 0, spread), reach, q)
+
+
+# ---------------------------------------------------------------------------------------------------------------- up to 8 rows
+#
+# A bound that knows what these rows are not rounded by. Of the result: half a step of fp16. Of the products p s, in two fp16 pieces: 2^-22
+# of each, or 2^-29 of the largest of the row and group, for each of n positions, times codes of 15 at most. Of fp32 sums of p m and p s c: 2^-16
+# of the sum of their sizes (2^8 of them after each other in one accumulator). Of the scores: sums of fp32 products, 2^-19 of scale sum |q| (|m| + 15 s),
+# which p is off by twice, relative.
+def held_sizes(cache, which, table, count, head):
+    """(step, |minimum|) float64 [count, groups] of positions 0..count-1."""
+    s = cache.ks if which == "k" else cache.vs
+    t = np.arange(count)
+    both = s[table[t // cache.page], head, :, t % cache.page].view(np.float16).astype(np.float64)
+    return both[..., 0], np.abs(both[..., 1])
+
+
+def exact_bound(cache, q, starts, lens, table, scale, want):
+    bound = np.full(want.shape, np.inf)
+    x, heads, kv = np.abs(q.astype(np.float64)), q.shape[1], cache.kc.shape[1]
+    for b in range(len(lens)):
+        for h in range(kv):
+            n = int(lens[b])
+            ks, km = held_sizes(cache, "k", table[b], n, h)
+            vs, vm = held_sizes(cache, "v", table[b], n, h)
+            keys, _ = cache.sequence("k", table[b], n, h)
+            for r in range(starts[b], starts[b + 1]):
+                upto = n - (starts[b + 1] - 1 - r)
+                for head in range(h * heads // kv, (h + 1) * heads // kv):
+                    score = keys[:upto] @ q[r, head].astype(np.float64) * scale
+                    p = np.exp(score - score.max())
+                    p /= p.sum()
+                    reach = (np.repeat(km[:upto] + 15 * ks[:upto], 32, 1) @ x[r, head]).max() * abs(scale)
+                    size = p @ (vm[:upto] + 15 * vs[:upto])
+                    largest = (p[:, None] * vs[:upto]).max(0)
+                    group = size * (2.0 ** -16 + 2.0 ** -22 + 2 * 2.0 ** -19 * reach) + 15 * upto * 2.0 ** -29 * largest
+                    bound[r, head] = 2.0 ** -11 * np.abs(want[r, head]) + 2.0 ** -25 + np.repeat(group, 32)
+    return bound
+
+
+def check_exact(got, cache, q, starts, lens, table, scale):
+    want, _, _ = plain.attend(cache, q, starts, lens, table, scale, 0)
+    err, bound = np.abs(got.astype(np.float64) - want), exact_bound(cache, q, starts, lens, table, scale, want)
+    assert np.isfinite(got).all()
+    assert (err <= bound).all(), (float((err / bound).max()), float((err - bound).max()))
+
+
+FEW = [(1, 4, 1), (1, 3, 1), (2, 4, 1), (1, 8, 1), (3, 4, 2), (4, 1, 1)]   # rows, heads, kv heads: up to 8 rows of a kv head
+
+
+@pytest.mark.parametrize("rows,heads,kv", FEW)
+@pytest.mark.parametrize("dim,bound", [(128, 300), (128, 5000), (64, 300), (64, 5000)])
+@pytest.mark.parametrize("how", ["alike", "groups", "positions", "any", "falling", "rising", "zeros"])
+def test_steps_of_different_sizes(torch_, how, dim, bound, rows, heads, kv):
+    """Steps of values of any sizes beside each other: in the groups of a position, from position to position (a large one that hardly counts
+    beside small ones that do), for rows that look at different positions, and with the scores that fall or rise."""
+    torch = torch_
+    rng = np.random.default_rng(dim + rows + heads + len(how))
+    page, lengths = 16, [bound if bound < 1000 else 1111, 70, rows]
+    cache, starts, lens, table = random_batch(rng, lengths, [rows] * 3, page, kv, dim)
+    shape = cache.vs.shape[:-1]
+    step = rng.uniform(0.1, 0.3, shape)
+    if how == "groups":
+        step = step * (2.0 ** np.array([14, -14, 0, -18]))[None, None, :dim // 32, None]
+    elif how in ("positions", "any"):
+        step = 2.0 ** rng.uniform(-20, 12, shape if how == "any" else shape[:2] + (1,) + shape[3:])
+    elif how in ("falling", "rising"):   # with the position: sizes from 2^12 to 2^-12
+        for b, n in enumerate(lengths):
+            t = np.arange(n)
+            power = np.linspace(12, -12, n)[::1 if how == "falling" else -1]
+            step[table[b, t // page], :, :, t % page] = (2.0 ** power)[:, None, None]
+    elif how == "zeros":
+        step = np.where(rng.integers(0, 3, shape) > 0, step, 0.0)
+    step = np.minimum(step, 4000.0)   # (m and m + 15 s are fp16 numbers)
+    set_scales(cache.vs, step, -step * rng.choice([0.0, 7.0, 15.0], shape))
+    # keys: rows prefer positions far apart, so that most of a row's positions hardly count
+    low = rng.choice([0.0, -0.3], cache.ks.shape[:-1])
+    set_scales(cache.ks, np.full(low.shape, 0.04), low)
+    q = (rng.standard_normal((3 * rows, heads, dim)) * rng.choice([1.0, 8.0, 30.0], (3 * rows, heads, 1))).astype(np.float16)
+    dev, batch = on_device(torch, cache, starts, lens, table)
+    check_exact(run(torch, q, dev, batch, rows, bound), cache, q, starts, lens, table, dim ** -0.5)
