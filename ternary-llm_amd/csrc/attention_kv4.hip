@@ -385,7 +385,8 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
         int step = tile.first_step + offset + wave;
         const int end = tile.first_step + offset + count;
         // row operands: this lane's row and its 8 dims of each group; and the groups' sums, which the minima multiply, as one
-        // more operand: first and second fp16 piece of sum / 32 at the depth of the quad that holds the minima of the row's tile
+        // more operand: first and second fp16 piece, times a power of two that brings the largest of the row's groups to 2^13 and
+        // more (small queries keep their bits beside large keys), at the depth of the quad that holds the minima of the row's tile
         // (rows that are not there are zeros; what they see shows in their own columns only)
         half8_t q[G], q_sums = {};
         {
@@ -403,20 +404,30 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
             at = find(step);
             load_keys(now, at);
         }
+        float c_sums[4];  // of this lane's rows: what undoes the power, and the scale
         {
+            float group_sum[G], largest = 0;
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                float sum = 0;
+                group_sum[g] = 0;
 #pragma unroll
-                for (int j = 0; j < 8; j++) sum += (float)q[g][j];
-                sum += __shfl_xor(sum, 16, kWave);
-                sum += __shfl_xor(sum, 32, kWave);
-                sum *= 0.03125f;
+                for (int j = 0; j < 8; j++) group_sum[g] += (float)q[g][j];
+                group_sum[g] += __shfl_xor(group_sum[g], 16, kWave);
+                group_sum[g] += __shfl_xor(group_sum[g], 32, kWave);
+                largest = fmaxf(largest, fabsf(group_sum[g]));
+            }
+            const int power = (__builtin_bit_cast(int, fminf(fmaxf(largest, 1e-30f), 1e30f)) >> 23) - 13;
+            const float by = as_float((254 - power) << 23);
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                const float sum = group_sum[g] * by;
                 if (quad == t16 / kRows * (kRows / 4)) {
                     q_sums[g] = (_Float16)sum;
                     q_sums[G + g] = (_Float16)(sum - (float)q_sums[g]);
                 }
             }
+#pragma unroll
+            for (int r = 0; r < 4; r++) c_sums[r] = as_float(__shfl(power, 4 * row_quad + r, kWave) << 23) * c_low;
         }
 
         float4_t acc[D::kSets][D::kNibbles];
@@ -529,7 +540,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
                         even = __builtin_fmaf(low_half(now.km[g]), d[g][r], even);
                         odd = __builtin_fmaf(low_half(now.km[g + 1]), d[g + 1][r], odd);
                     }
-                    raw[r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low[r] * (32.0f * c_low)));
+                    raw[r] = __builtin_fmaf(even, c_even, __builtin_fmaf(odd, c_odd, low[r] * c_sums[r]));
                 }
                 if (!whole) {
                     asm volatile("");

@@ -142,3 +142,21 @@ def test_steps_of_different_sizes(torch_, how, dim, bound, rows, heads, kv):
     q = (rng.standard_normal((3 * rows, heads, dim)) * rng.choice([1.0, 8.0, 30.0], (3 * rows, heads, 1))).astype(np.float16)
     dev, batch = on_device(torch, cache, starts, lens, table)
     check_exact(run(torch, q, dev, batch, rows, bound), cache, q, starts, lens, table, dim ** -0.5)
+
+
+@pytest.mark.parametrize("rows,heads,kv", FEW[:4])
+@pytest.mark.parametrize("power", [-15, -11, -7, 5])
+@pytest.mark.parametrize("dim,bound", [(128, 300), (64, 5000)])
+def test_small_queries_and_large_keys(torch_, dim, bound, power, rows, heads, kv):
+    """Scores of some units from queries of 2^-15 and keys of 2^15, and the other way round; rows of very different sizes in a tile."""
+    torch = torch_
+    rng = np.random.default_rng(dim + rows + heads + power)
+    lengths = [300, 70]
+    cache, starts, lens, table = random_batch(rng, lengths, [rows] * 2, 16, kv, dim)
+    step = 2.0 ** (-power - 4) * rng.uniform(0.5, 1.0, cache.ks.shape[:-1])
+    set_scales(cache.ks, step, -step * rng.choice([0.0, 7.5, 15.0], step.shape))
+    q = rng.standard_normal((2 * rows, heads, dim)) * 2.0 ** power
+    q[:, 0] *= 2.0 ** -6
+    q = q.astype(np.float16)
+    dev, batch = on_device(torch, cache, starts, lens, table)
+    check_exact(run(torch, q, dev, batch, rows, bound), cache, q, starts, lens, table, dim ** -0.5)
