@@ -379,6 +379,9 @@ int tllm_kv4_read_f16(uint16_t *k, uint16_t *v, int64_t k_stride, int64_t v_stri
  * Few row tiles over long contexts are shared out along the positions and joined through it. It depends on the
  * sizes and on the current device, not on the arrays' contents. Negative: a TLLM_ERR_* code.
  * Limits: n_heads a multiple of n_kv_heads, <= 4096; 1 <= max_query, max_length; n_heads * max_query <= 2^27; |scale| <= 2^40.
+ * Row tiles, and steps of positions of all of them, are counted in 32 bits, for any contents of the arrays. Where a count might
+ * not fit the call is TLLM_ERR_TOO_LARGE; it fits with max_length <= 2^29, batch * max_length < 2^34 and batch * max_query * n_heads /
+ * n_kv_heads < 2^38.
  * The reference's counterpart for an fp16 cache is kernels/attention.cu:30-333.
  */
 int64_t tllm_attention_kv4_workspace_bytes(const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, int n_heads, int max_query,

@@ -1673,6 +1673,19 @@ Plans plans_of(const AttentionKv4Args &a) {
     return p;
 }
 
+// The kernels count row tiles, and in line the steps of positions of all of them, in 32 bits (as many as the sizes allow, whatever
+// the arrays hold), and the counts are rounded up to whole grids and pieces.
+template <int kDim>
+bool counts_fit(const AttentionKv4Args &a) {
+    const Plans p = plans_of<kDim>(a);
+    const auto fits = [&](const RowPlan &plan, int step) {
+        const long long numbers = (long long)a.batch.batch * plan.tiles, steps = (a.max_length - 1) / step + 1;
+        return (plan.alone ? numbers : numbers * steps) < INT32_MAX - (1 << 16);
+    };
+    return (!p.few || fits(p.few_plan, p.few_rows == 4 ? Decode<kDim, 4>::kStep : Decode<kDim, 8>::kStep)) &&
+           (!p.many || fits(p.many_plan, Prompt<kDim, kPromptWaves>::kTile));
+}
+
 dim3 worker_grid(const AttentionKv4Args &a, const RowPlan &plan) {
     const int across = std::min(plan.workers, 32768);
     return dim3((unsigned)a.cache.n_kv_heads, (unsigned)across, (unsigned)((plan.workers + across - 1) / across));
@@ -1737,6 +1750,8 @@ hipError_t launch(const AttentionKv4Args &a, hipStream_t s) {
 }
 
 }  // namespace
+
+bool attention_kv4_fits(const AttentionKv4Args &a) { return a.cache.head_dim == 64 ? counts_fit<64>(a) : counts_fit<128>(a); }
 
 size_t attention_kv4_workspace(const AttentionKv4Args &a) {
     const Plans p = a.cache.head_dim == 64 ? plans_of<64>(a) : plans_of<128>(a);

@@ -423,14 +423,10 @@ static int attention_kv4_args(const tllm_kv4_cache *cache, const tllm_kv4_batch 
     if (n_heads < 1 || n_heads % a->cache.n_kv_heads || max_query < 1 || max_length < 1) return TLLM_ERR_BAD_SHAPE;
     if (n_heads > 4096 || (int64_t)n_heads * std::min(max_query, a->batch.n_tokens) > 1 << 27) return TLLM_ERR_TOO_LARGE;
     const int capacity = a->batch.width << a->cache.page_shift;
-    // (the kernels count the steps of positions of all row tiles in 32 bits: at most 17 tiles of few rows a sequence, in steps of 32
-    // or more positions, or tiles of 128 rows)
-    const int64_t rows = (int64_t)std::min(max_query, a->batch.n_tokens) * (n_heads / a->cache.n_kv_heads);
-    if ((rows / 128 + 17) * a->batch.batch * (std::min(max_length, capacity) / 32 + 1) > INT32_MAX) return TLLM_ERR_TOO_LARGE;
     a->n_heads = n_heads;
     a->max_query = max_query < a->batch.n_tokens ? max_query : a->batch.n_tokens;
     a->max_length = max_length < capacity ? max_length : capacity;
-    return TLLM_OK;
+    return tllm::attention_kv4_fits(*a) ? TLLM_OK : TLLM_ERR_TOO_LARGE;
 }
 
 int64_t tllm_attention_kv4_workspace_bytes(const tllm_kv4_cache *cache, const tllm_kv4_batch *batch, int n_heads, int max_query,

@@ -184,7 +184,9 @@ struct AttentionKv4Args {
     float scale;
     void *workspace;
 };
-size_t attention_kv4_workspace(const AttentionKv4Args &a);  // pointers are not looked at
+// Neither looks at pointers. Whether the sizes' row tiles and steps can be counted; bytes for any window.
+bool attention_kv4_fits(const AttentionKv4Args &a);
+size_t attention_kv4_workspace(const AttentionKv4Args &a);
 hipError_t launch_attention_kv4(const AttentionKv4Args &a, hipStream_t s);
 
 // Measurement aid (elementwise.hip): reads `bytes` of device memory once.
