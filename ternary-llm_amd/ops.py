@@ -326,6 +326,13 @@ def _want(cond, text):
         raise ValueError(text)
 
 
+def _in_int32(**values):
+    """ctypes cuts a larger number to its low 32 bits without a word."""
+    for name, value in values.items():
+        if not -2 ** 31 <= value < 2 ** 31:
+            raise ValueError(f"{name} does not fit 32 bits")
+
+
 def _rows(t, name, heads=None):
     """A tensor of rows [n, heads, dim]: fp16, heads next to each other; returns its row stride in elements."""
     if t.dim() != 3 or t.dtype != _torch().float16:
@@ -385,6 +392,7 @@ def rotary(q, k, q_out, k_out, positions, rotary_dim, theta, layout="interleaved
         kv_heads = k.shape[1]
         _want(k.shape == k_out.shape and k.shape[0] == n and k.shape[2] == dim, "k and k_out must have q's rows and dim")
     _want(_is_int32(positions) and positions.shape == (n,), "positions must be a contiguous int32 [rows]")
+    _in_int32(rotary_dim=rotary_dim, original_length=original_length)
     if high_turns is None:
         high_turns = 32.0 if scaling == "yarn" else 4.0
     config = _RotaryConfig(rotary_dim, ROTARY_LAYOUTS[layout], ROTARY_SCALINGS[scaling], original_length, theta, factor, low_turns,
@@ -453,6 +461,7 @@ def attention_kv4(q, output, k_codes, k_scales, v_codes, v_scales, query_starts,
     cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n)
     qs, os_ = _rows(q, "q"), _rows(output, "output")
     _want(output.shape == q.shape and dim == cache.head_dim, "q and output must be [rows, heads, dim] with the cache's dim")
+    _in_int32(max_query=max_query, max_length=max_length, window=window)
     if scale is None:
         scale = dim ** -0.5
 
@@ -480,6 +489,7 @@ def attention_kv4_workspace_bytes(n_heads, k_codes, k_scales, v_codes, v_scales,
                                   max_length):
     """Bytes of workspace that attention_kv4 uses for these sizes on the current device."""
     cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n_rows)
+    _in_int32(n_heads=n_heads, n_rows=n_rows, max_query=max_query, max_length=max_length)
     need = int(lib().tllm_attention_kv4_workspace_bytes(cache, batch, n_heads, max_query, max_length))
     if need < 0:
         check(need)

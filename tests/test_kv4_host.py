@@ -2,6 +2,8 @@
 import os
 import subprocess
 
+import pytest
+
 import ternary_llm_amd as tl
 from tests.test_kv4 import _attend_call, _kv4
 
@@ -34,3 +36,26 @@ def test_attention_takes_all_sizes_that_it_can_count():
     assert size(64, 1, 1 << 21, 16, n=1 << 23, width=1, **wide) == -4                    # 2^43: 2^35 row tiles
     # the call itself refuses them too, before it looks at anything on the device
     assert _attend_call(heads=8, kv_heads=1, qs=512, os_=512, mq=1, ml=1 << 30, n=65535, width=1 << 17, pages=1000, page=16, batch=65535) == -4
+
+
+def test_numbers_beyond_32_bits():
+    """A window of 2^32 is not none, a bound of 2^32 + 1 not one position."""
+    import torch
+    q = torch.zeros(3, 4, 64, dtype=torch.float16)
+    pos = torch.zeros(3, dtype=torch.int32)
+    cache = tl.kv4_cache(4, 16, 4, 64, device="cpu")
+    batch = (torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, dtype=torch.int32))
+    for wrong in (2 ** 31, 2 ** 32 + 1, -2 ** 31 - 1):
+        with pytest.raises(ValueError, match="window"):
+            tl.attention_kv4(q, q.clone(), *cache, *batch, 3, 32, window=wrong)
+        with pytest.raises(ValueError, match="max_length"):
+            tl.attention_kv4(q, q.clone(), *cache, *batch, 3, wrong)
+        with pytest.raises(ValueError, match="max_query"):
+            tl.attention_kv4(q, q.clone(), *cache, *batch, wrong, 32)
+        for name, numbers in (("n_heads", (wrong, 3, 3, 32)), ("n_rows", (4, wrong, 3, 32)), ("max_query", (4, 3, wrong, 32)), ("max_length", (4, 3, 3, wrong))):
+            with pytest.raises(ValueError, match=name):
+                tl.attention_kv4_workspace_bytes(numbers[0], *cache, *batch, *numbers[1:])
+        with pytest.raises(ValueError, match="rotary_dim"):
+            tl.rotary(q, None, q, None, pos, wrong, 1e4)
+        with pytest.raises(ValueError, match="original_length"):
+            tl.rotary(q, None, q, None, pos, 64, 1e4, scaling="yarn", original_length=wrong)
