@@ -329,7 +329,7 @@ def _want(cond, text):
 def _in_int32(**values):
     """ctypes cuts a larger number to its low 32 bits without a word."""
     for name, value in values.items():
-        if not -2 ** 31 <= value < 2 ** 31:
+        if value + 0x80000000 >> 32:
             raise ValueError(f"{name} does not fit 32 bits")
 
 
@@ -461,7 +461,8 @@ def attention_kv4(q, output, k_codes, k_scales, v_codes, v_scales, query_starts,
     cache, batch = _kv4(k_codes, k_scales, v_codes, v_scales, query_starts, lengths, page_table, n)
     qs, os_ = _rows(q, "q"), _rows(output, "output")
     _want(output.shape == q.shape and dim == cache.head_dim, "q and output must be [rows, heads, dim] with the cache's dim")
-    _in_int32(max_query=max_query, max_length=max_length, window=window)
+    if (max_query + 0x80000000 | max_length + 0x80000000 | window + 0x80000000) >> 32:
+        _in_int32(max_query=max_query, max_length=max_length, window=window)
     if scale is None:
         scale = dim ** -0.5
 
