@@ -634,6 +634,9 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_decode_kernel(cons
                         for (int j = 0; j < 2; j++) {
                             float one = w[2 * j] * size[g], two = w[2 * j + 1] * size[g];
                             if constexpr (kEach) one *= as_float(lift[g][2 * j]), two *= as_float(lift[g][2 * j + 1]);
+                            // (rounded to fp32 here: a product that is rounded to fp16 at once, beside one that is not, makes the second piece
+                            // that of another first piece, a step off, where the fp32 product lies half-way between two fp16 numbers)
+                            asm("" : "+v"(one), "+v"(two));
                             const half2_t h = {(_Float16)one, (_Float16)two};
                             const half2_t l = {(_Float16)__builtin_fmaf((float)h[0], minus_one, one), (_Float16)__builtin_fmaf((float)h[1], minus_one, two)};
                             hi[j] = __builtin_bit_cast(uint32_t, h);
