@@ -377,7 +377,8 @@ int tllm_kv4_read_f16(uint16_t *k, uint16_t *v, int64_t k_stride, int64_t v_stri
  * workspace: tllm_attention_kv4_workspace_bytes() bytes of device memory, 16-byte aligned (NULL when that is 0), used during
  * the call only, contents do not matter; calls that may overlap in time need one each. TLLM_ERR_SCRATCH_TOO_SMALL if less.
  * Few row tiles over long contexts are shared out along the positions and joined through it. It depends on the
- * sizes and on the current device, not on the arrays' contents. Negative: a TLLM_ERR_* code.
+ * sizes and on the current device, not on the arrays' contents, and suffices for any window (a call with one may use less).
+ * Negative: a TLLM_ERR_* code.
  * Limits: n_heads a multiple of n_kv_heads, <= 4096; 1 <= max_query, max_length; n_heads * max_query <= 2^27; |scale| <= 2^40.
  * Row tiles, and steps of positions of all of them, are counted in 32 bits, for any contents of the arrays. Where a count might
  * not fit the call is TLLM_ERR_TOO_LARGE; it fits with max_length <= 2^29, batch * max_length < 2^34 and batch * max_query * n_heads /

@@ -120,7 +120,7 @@ __device__ __forceinline__ int position_limit(const AttentionKv4Args &a) { retur
 // second launch. A wave is a workgroup of its own: nothing waits for another wave. The other form, for short contexts or
 // many sequences (see plans_of): a workgroup of kAloneWaves waves has a whole row tile, the waves take its steps in turn and
 // meet in LDS, and there is no second launch.
-// Measured (32 query heads, 8 kv heads of 128 dims): 32 sequences of 4096 positions 32 us, a read of their 5 bits 28; the
+// Measured (32 query heads, 8 kv heads of 128 dims): 32 sequences of 4096 positions 33 us, a read of their 5 bits 28; the
 // line, 72 000 positions of 32 ragged sequences: 29 us and 5 for the joins, a read 15; 131 072 positions of one sequence with
 // 64 heads: 41 and 6, a read 28. What is left is the vector pipe (some 800 instructions a step of 64 positions, two waves a
 // SIMD for the registers) and, in the line, the chain of loads before a wave's first step and behind its last.
@@ -897,7 +897,7 @@ __device__ __forceinline__ uint32_t values_of(uint32_t field, bool odd, uint32_t
 // operand has dims as rows: a lane has one word's dims of 16 positions, and of the row tiles' order only the stores know. k, v
 // and p are rounded to fp16 (see the next section).
 // Measured (32 heads, 8 kv heads of 128): five drafts for 16 users in a window of 1024 18 us as whole row tiles, 36 in line;
-// 16 sequences of 8192 positions with 32 rows each 73 us, with 64 rows 109, a read of the cache 28.
+// 16 sequences of 8192 positions with 32 rows each 74 us, with 64 rows 111, a read of the cache 28.
 template <int kDim>
 struct Rows32 {
     static constexpr int kGroups = kDim / kKvGroup, kWords = kDim / 8;
@@ -1488,7 +1488,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
                 float16_t x[P::kSub];
                 float most = -INFINITY;
                 // (the order written here is kept: a read of LDS 4 matrix instructions ahead of its use. Left to itself the compiler
-                // puts each read right before its use, and both waves of a SIMD wait for LDS half the time: a prompt of 4096 takes 180 us, 171 so)
+                // puts each read right before its use, and both waves of a SIMD wait for LDS half the time: a prompt of 4096 takes 180 us, 170 so)
                 constexpr int kReads = P::kSub * P::kDepths, kAhead = 4;
                 const auto key = [&](int at) { return *(const half8_t *)(keys + 32 * (at / P::kDepths) * P::kKeyBytes + at % P::kDepths * 32); };
                 half8_t ahead[kAhead];
@@ -1608,7 +1608,7 @@ __global__ __launch_bounds__(kWaves *kWave, 2) void attention_prompt_kernel(cons
 // ------------------------------------------------------------------------------------------------- launches
 
 // Rows (query rows times heads of a kv head) up to which a sequence goes the way of few rows. 16 sequences of 8192 positions,
-// 64 rows each: 109 us, 138 as a prompt; 128 rows: 181 and 140. (One sequence of 8192 positions, 64 rows: 35 and 20.)
+// 64 rows each: 111 us, 138 as a prompt; 128 rows: 181 and 140. (One sequence of 8192 positions, 64 rows: 35 and 20.)
 constexpr int kFewRows = 64;
 
 // Rows of a tile: 4 and 8 take bare codes, 32 values brought to fp16. 8 rows, 131 072 positions: 47 us with 8, 56 with 32; 4
