@@ -369,11 +369,11 @@ int tllm_kv4_read_f16(uint16_t *k, uint16_t *v, int64_t k_stride, int64_t v_stri
  * max_query and max_length are upper bounds the host knows: rows of a sequence from max_query on are left as they were, positions from
  * max_length on are not seen. They size the launch, so tight ones are faster; for a captured graph take the largest of
  * its replays. The same call gives the same bits.
- * Scores, softmax statistics and sums are fp32. Up to 8 rows of a kv head (a sequence's rows times n_heads / n_kv_heads)
- * multiply q with the codes themselves and take weights times steps in two fp16 pieces: next to the result's own rounding
- * these are rounded by 2^-22, or 2^-29 of the largest of their row and group of dims, and nothing else to fewer than 32 bits.
- * From 9 rows on k and v are what tllm_kv4_read_f16 gives (one rounding to fp16, kept within +-65504), and p is rounded to
- * fp16 (2^-11; weights below 2^-20 of a row's largest to 2^-31 of it) before their products.
+ * Scores, softmax statistics and sums are fp32. A call with up to 8 rows of a kv head (max_query, n_tokens at most, times
+ * n_heads / n_kv_heads) multiplies q with the codes themselves and takes weights times steps in two fp16 pieces: next to the
+ * result's own rounding these are rounded by 2^-22, or 2^-29 of the largest of their row and group of dims, and nothing else to
+ * fewer than 32 bits. In a call with more, for all its sequences, k and v are what tllm_kv4_read_f16 gives (one rounding to fp16,
+ * kept within +-65504), and p is rounded to fp16 (2^-11; weights below 2^-20 of a row's largest to 2^-31 of it) before their products.
  * workspace: tllm_attention_kv4_workspace_bytes() bytes of device memory, 16-byte aligned (NULL when that is 0), used during
  * the call only, contents do not matter; calls that may overlap in time need one each. TLLM_ERR_SCRATCH_TOO_SMALL if less.
  * Few row tiles over long contexts are shared out along the positions and joined through it. It depends on the
